@@ -165,6 +165,41 @@ class Wino3dParams(C.Structure):
                 ("alpha", c_f32), ("frame_rows", c_i32), ("row_offset", c_i32), ("tiles_ld", c_i32)]
 
 
+class RotaryParams(C.Structure):
+    _fields_ = [("x", c_vp), ("y", c_vp), ("pos", c_vp), ("freq", c_vp), ("sx_row", c_i64), ("sx_head", c_i64), ("sy_row", c_i64), ("sy_head", c_i64),
+                ("rows", c_i32), ("heads", c_i32), ("hd", c_i32), ("rot", c_i32), ("interleaved", c_i32), ("backward", c_i32), ("f32", c_i32), ("mscale", c_f32)]
+
+
+class PageTablesParams(C.Structure):
+    _fields_ = [("ctx_len", c_vp), ("new_len", c_vp), ("held", c_vp), ("free_pages", c_vp), ("table", c_vp), ("kv_len", c_vp), ("cu_q", c_vp),
+                ("slots", c_vp), ("pos", c_vp), ("held_out", c_vp), ("taken", c_vp), ("ld_table", c_i64),
+                ("requests", c_i32), ("max_pages", c_i32), ("page", c_i32), ("rows", c_i32), ("n_free", c_i32)]
+
+
+class Kv4AppendParams(C.Structure):
+    _fields_ = [("k", c_vp), ("v", c_vp), ("codes", c_vp), ("scales", c_vp), ("slots", c_vp),
+                ("sk_row", c_i64), ("sk_head", c_i64), ("sv_row", c_i64), ("sv_head", c_i64),
+                ("rows", c_i32), ("kv", c_i32), ("hd", c_i32), ("page", c_i32), ("pages", c_i32)]
+
+
+class Kv4ReadParams(C.Structure):
+    _fields_ = [("codes", c_vp), ("scales", c_vp), ("slots", c_vp), ("k", c_vp), ("v", c_vp),
+                ("rows", c_i32), ("kv", c_i32), ("hd", c_i32), ("page", c_i32), ("pages", c_i32), ("f32", c_i32)]
+
+
+class Kv4AttnParams(C.Structure):
+    _fields_ = [("q", c_vp), ("codes", c_vp), ("scales", c_vp), ("table", c_vp), ("kv_len", c_vp), ("cu_q", c_vp), ("out", c_vp), ("partial", c_vp),
+                ("sq_row", c_i64), ("sq_head", c_i64), ("so_row", c_i64), ("ld_table", c_i64),
+                ("requests", c_i32), ("heads", c_i32), ("kv", c_i32), ("hd", c_i32), ("page", c_i32), ("pages", c_i32), ("max_pages", c_i32),
+                ("rows", c_i32), ("max_q", c_i32), ("n_split", c_i32), ("alpha", c_f32)]
+
+
+class VerifyDraftsParams(C.Structure):
+    _fields_ = [("draft", c_vp), ("q", c_vp), ("p", c_vp), ("u", c_vp), ("pick", c_vp), ("count", c_vp), ("tokens", c_vp), ("accepted", c_vp),
+                ("sq_req", c_i64), ("sq_row", c_i64), ("sp_req", c_i64), ("sp_row", c_i64),
+                ("requests", c_i32), ("drafts", c_i32), ("vocab", c_i32), ("bf16", c_i32)]
+
+
 class GemmWorkspace(C.Structure):
     _fields_ = [("image", c_vp), ("image_bytes", C.c_size_t), ("scratch", c_vp), ("scratch_bytes", C.c_size_t)]
 
@@ -184,6 +219,8 @@ STRUCTS = {
     "grove_normalize_params": NormalizeParams, "grove_gemm_f32_params": GemmF32Params, "grove_gemm_fp8_params": GemmFp8Params,
     "grove_gemm_workspace": GemmWorkspace, "grove_gemm_plan": GemmPlan, "grove_greedy_pick_params": GreedyPickParams,
     "grove_wino3d_params": Wino3dParams,
+    "grove_rotary_params": RotaryParams, "grove_page_tables_params": PageTablesParams, "grove_kv4_append_params": Kv4AppendParams,
+    "grove_kv4_read_params": Kv4ReadParams, "grove_kv4_attn_params": Kv4AttnParams, "grove_verify_drafts_params": VerifyDraftsParams,
 }
 
 # every symbol include/grove_hip.h declares (tests/test_abi.py checks the header against this list)
@@ -196,6 +233,7 @@ SYMBOLS = [
     "grove_im2col_patch", "grove_clip_pool", "grove_cross_entropy", "grove_small_attn_fwd", "grove_small_attn_bwd", "grove_small_attn_set_tiny", "grove_small_attn_bwd_stores_bf16", "grove_gemm_f32", "grove_gemm_fp8", "grove_gemm_fp8_set_pipelined", "grove_quant_fp8_rows", "grove_quant_fp8_rows_act",
     "grove_box_head_fwd", "grove_box_head_bwd", "grove_box_losses", "grove_adamw_step", "grove_adamw_step_multi", "grove_sumsq_f32",
     "grove_wino3d_transform_tokens", "grove_wino3d_transform_weight", "grove_wino3d_output", "grove_wino3d_wgrad_output",
+    "grove_rotary", "grove_page_tables", "grove_kv4_append", "grove_kv4_read", "grove_kv4_attn", "grove_verify_drafts",
 ]
 
 _lib = None

@@ -72,6 +72,12 @@ extern "C" int grove_sizeof(const char* name) {
   SZ(grove_gemm_workspace);
   SZ(grove_gemm_plan);
   SZ(grove_wino3d_params);
+  SZ(grove_rotary_params);
+  SZ(grove_page_tables_params);
+  SZ(grove_kv4_append_params);
+  SZ(grove_kv4_read_params);
+  SZ(grove_kv4_attn_params);
+  SZ(grove_verify_drafts_params);
 #undef SZ
   return -1;
 }

@@ -5,7 +5,9 @@ hand-written gfx950 kernels in grove_amd/csrc. Nothing in this module falls back
 Tensors are bf16 unless stated; every function launches on torch's current stream.
 """
 import ctypes as C
+import math
 import os
+from typing import NamedTuple
 
 import torch
 
@@ -1176,3 +1178,270 @@ def sumsq(x, out=None):
         out = torch.zeros(1, dtype=torch.float32, device=x.device)
     _lib.check(_lib.lib().grove_sumsq_f32(_p(x), _p(out), C.c_int64(x.numel()), _stream()), "grove_sumsq_f32")
     return out
+
+
+# ---- serving from a paged 4-bit cache with drafted tokens (grove_hip.h "Serving from a paged 4-bit key / value cache")
+def _need(cond, what, msg):
+    if not cond:
+        raise RuntimeError(f"{what}: {msg}")
+
+
+def _one_device(what, *ts):
+    """Every tensor on the CURRENT device: a launch goes to it, whatever device its tensors are on."""
+    _chk_dev(*ts)
+    cur = torch.cuda.current_device()
+    for t in ts:
+        _need(t is None or t.device.index == cur, what, f"a tensor is on {t.device if t is not None else None}, the current device is cuda:{cur}")
+
+
+def _lens(what, n, **ts):
+    for name, t in ts.items():
+        _need(t.dtype == torch.int32 and t.dim() == 1 and t.shape[0] == n and t.is_contiguous(), what, f"{name} must be contiguous int32 [{n}]")
+
+
+def _span(t):
+    """(first byte, byte behind the last) of a tensor's elements."""
+    last = sum((n - 1) * s for n, s in zip(t.shape, t.stride())) if t.numel() else -1
+    return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+
+
+def _apart(a, b):
+    (a0, a1), (b0, b1) = _span(a), _span(b)
+    return a1 <= b0 or b1 <= a0
+
+
+def _own_elements(t):
+    """No two elements of a view share memory (a broadcast view must not be written)."""
+    at = 1
+    for s, n in sorted((s, n) for s, n in zip(t.stride(), t.shape) if n > 1):
+        if s < at:
+            return False
+        at = s * n
+    return True
+
+
+class RotaryPlan(NamedTuple):
+    """freq: f64 [rot / 2] on the device, radians per position of each pair; interleaved: pairs (2 i, 2 i + 1) instead of (i, i + rot / 2);
+    mscale: factor on the rotated channels. Made once per model by rotary_plan."""
+    freq: torch.Tensor
+    interleaved: bool = False
+    mscale: float = 1.0
+
+
+def rotary_plan(rot, theta=10000.0, *, interleaved=False, scaling="none", factor=1.0, trained_len=4096, fast=32.0, slow=1.0, device="cuda"):
+    """The frequencies theta^(-2 i / rot) of `rot` rotated channels, stretched by `factor` for contexts longer than `trained_len`:
+    "linear" divides every frequency; "ntk" raises theta to theta * factor^(rot / (rot - 2)), which divides the lowest frequency only; "yarn"
+    divides the pairs that turn less than `slow` times in trained_len, leaves those that turn more than `fast` times, blends linearly over
+    the pair number between, and scales the rotated channels by 0.1 ln(factor) + 1 (Peng et al. 2023)."""
+    what = "rotary_plan"
+    _need(rot >= 2 and rot % 2 == 0, what, f"rot = {rot} must be even and positive")
+    _need(scaling in ("none", "linear", "ntk", "yarn"), what, f"unknown scaling {scaling!r}")
+    _need(theta > 1.0 and factor >= 1.0, what, "theta must pass 1 and factor must not be below 1")
+    _need(scaling != "none" or factor == 1.0, what, "a factor needs a scaling")
+    mscale = 1.0
+    if scaling == "ntk":
+        _need(rot > 2, what, "ntk needs rot > 2")
+        theta = theta * factor ** (rot / (rot - 2))
+    w = theta ** -(torch.arange(0, rot, 2, dtype=torch.float64) / rot)
+    if scaling == "linear":
+        w = w / factor
+    elif scaling == "yarn":
+        _need(trained_len > 0 and fast > slow > 0, what, "yarn needs trained_len > 0 and fast > slow > 0")
+
+        def pair(turns):  # the (real) pair number, times two, that turns so many times in trained_len
+            return rot * math.log(trained_len / (turns * 2 * math.pi)) / (2 * math.log(theta))
+        low, high = max(math.floor(pair(fast)), 0), min(math.ceil(pair(slow)), rot - 1)
+        ramp = ((torch.arange(rot // 2, dtype=torch.float64) - low) / max(high - low, 0.001)).clamp(0, 1)
+        w = w / factor * ramp + w * (1 - ramp)
+        mscale = 0.1 * math.log(factor) + 1.0
+    return RotaryPlan(w.to(device), bool(interleaved), mscale)
+
+
+def rotary(x, pos, plan, *, backward=False, out=None):
+    """Rotary positions of x [rows, heads, hd] (bf16 or f32, any row and head strides: q and k of a packed projection in one call) at pos int32
+    [rows] (grove_rotary). out None: a new tensor; out = x (the same view): in place; any other out must not overlap x. backward: the gradient
+    w.r.t. x for x = the gradient w.r.t. the result."""
+    what = "rotary"
+    _need(x.dim() == 3 and x.dtype in (bf16, torch.float32), what, "x must be bf16 or f32 [rows, heads, hd]")
+    rows, heads, hd = x.shape
+    _need(x.stride(2) == 1 or hd == 1 or x.numel() == 0, what, "the channels must be contiguous")
+    f = plan.freq
+    _need(f.dtype == torch.float64 and f.dim() == 1 and f.is_contiguous() and 0 < 2 * f.shape[0] <= hd, what, f"the plan must hold 1 to {hd // 2} f64 frequencies")
+    _lens(what, rows, pos=pos)
+    if out is None:
+        _chk_dev(x)
+        out = torch.empty((rows, heads, hd), dtype=x.dtype, device=x.device)
+    else:
+        _need(out.shape == x.shape and out.dtype == x.dtype and (out.stride(2) == 1 or out.numel() == 0), what, "out must match x, its channels contiguous")
+        _need(_own_elements(out), what, "out has elements that share memory")
+        same = out.data_ptr() == x.data_ptr() and out.stride() == x.stride()
+        _need(same or _apart(out, x), what, "out overlaps x and is not the same view")
+    _one_device(what, x, pos, f, out)
+    p = _lib.RotaryParams()
+    p.x, p.y, p.pos, p.freq = _p(x), _p(out), _p(pos), _p(f)
+    p.sx_row, p.sx_head, p.sy_row, p.sy_head = x.stride(0), x.stride(1), out.stride(0), out.stride(1)
+    p.rows, p.heads, p.hd, p.rot = rows, heads, hd, 2 * f.shape[0]
+    p.interleaved, p.backward, p.f32, p.mscale = int(plan.interleaved), int(backward), int(x.dtype == torch.float32), float(plan.mscale)
+    _lib.check(_lib.lib().grove_rotary(C.byref(p), _stream()), "grove_rotary")
+    return out
+
+
+class PageStep(NamedTuple):
+    """What page_tables makes of a step: kv_len [requests], cu_q [requests + 1], slots [rows], pos [rows], held [requests], taken [1], all int32."""
+    kv_len: torch.Tensor
+    cu_q: torch.Tensor
+    slots: torch.Tensor
+    pos: torch.Tensor
+    held: torch.Tensor
+    taken: torch.Tensor
+
+
+def page_tables(ctx_len, new_len, table, held, free, page_size, rows):
+    """Hands pages to the requests of a step and maps its rows to slots, in one launch (grove_page_tables). ctx_len, new_len, held: int32
+    [requests] tokens in the cache, tokens of this step, pages a request has; table: int32 [requests, max_pages], changed in place; free: int32
+    page numbers, used from the front; rows: the rows of the step, sum(new_len), or more for a step of fixed size. The caller drops the first
+    `taken` of `free` (taken > len(free): the pages ran out, the rows without a page have slot -1)."""
+    what = "page_tables"
+    _need(table.dim() == 2 and table.dtype == torch.int32 and table.shape[0] > 0 and table.shape[1] > 0 and table.stride(1) == 1 and _own_elements(table),
+          what, "table must be int32 [requests, max_pages], its rows contiguous and apart")
+    B = table.shape[0]
+    _lens(what, B, ctx_len=ctx_len, new_len=new_len, held=held)
+    _need(free.dtype == torch.int32 and free.dim() == 1 and free.is_contiguous(), what, "free must be contiguous int32")
+    _need(B <= 4096, what, f"{B} requests: at most 4096")
+    _need(page_size >= 1 and page_size & (page_size - 1) == 0, what, "the page size must be a power of two")
+    _need(0 <= rows < 2 ** 31, what, "bad number of rows")
+    _need(all(_apart(table, t) for t in (ctx_len, new_len, held, free)), what, "table overlaps an input")
+    _one_device(what, ctx_len, new_len, table, held, free)
+    o = torch.empty(3 * B + 2 + 2 * rows, dtype=torch.int32, device=table.device)  # one allocation for the six results
+    step = PageStep(*o.split([B, B + 1, rows, rows, B, 1]))
+    p = _lib.PageTablesParams()
+    p.ctx_len, p.new_len, p.held, p.free_pages, p.table = _p(ctx_len), _p(new_len), _p(held), _p(free), _p(table)
+    p.kv_len, p.cu_q, p.slots, p.pos, p.held_out, p.taken = (_p(t) for t in step)
+    p.ld_table = max(table.stride(0), table.shape[1])
+    p.requests, p.max_pages, p.page, p.rows, p.n_free = B, table.shape[1], page_size, rows, free.shape[0]
+    _lib.check(_lib.lib().grove_page_tables(C.byref(p), _stream()), "grove_page_tables")
+    return step
+
+
+class KV4Cache(NamedTuple):
+    """The pages of one layer's 4-bit cache (layout: grove_hip.h): codes uint8 [pages, 2, kv, page_size * hd / 2], scales bf16
+    [pages, 2, kv, page_size, 2]. 4.25 bits a channel at hd = 128."""
+    codes: torch.Tensor
+    scales: torch.Tensor
+
+
+def kv4_cache(pages, page_size, kv, hd, device):
+    """An empty 4-bit cache of `pages` pages for `kv` key / value heads of hd channels."""
+    _need(page_size in (16, 32, 64, 128, 256) and hd in (32, 64, 128, 256), "kv4_cache", "the page must hold 16 to 256 tokens, the head 32, 64, 128 or 256 channels")
+    return KV4Cache(torch.zeros((pages, 2, kv, page_size * hd // 2), dtype=torch.uint8, device=device),
+                    torch.zeros((pages, 2, kv, page_size, 2), dtype=bf16, device=device))
+
+
+def _kv4_shape(what, cache):
+    """(pages, kv, page_size, hd) of a cache."""
+    c, s = cache
+    _need(c.dtype == torch.uint8 and c.dim() == 4 and c.is_contiguous() and s.dtype == bf16 and s.dim() == 5 and s.is_contiguous(), what,
+          "the cache must be a KV4Cache of contiguous tensors")
+    pages, two, kv, P = s.shape[:4]
+    _need(two == 2 and s.shape[4] == 2 and c.shape[:3] == s.shape[:3] and pages > 0 and kv > 0 and P in (16, 32, 64, 128, 256), what, "codes and scales do not fit each other")
+    hd = 2 * c.shape[3] // P
+    _need(hd in (32, 64, 128, 256) and hd * P == 2 * c.shape[3], what, "the head must have 32, 64, 128 or 256 channels")
+    return pages, kv, P, hd
+
+
+def kv4_append(k, v, cache, slots):
+    """Quantises the rows of k and v (bf16 [rows, kv, hd], any row and head strides) into the cache rows `slots` (int32 [rows], page *
+    page_size + offset; one outside the cache is skipped, the others are distinct) (grove_kv4_append)."""
+    what = "kv4_append"
+    pages, kv, P, hd = _kv4_shape(what, cache)
+    for t in (k, v):
+        _need(t.dtype == bf16 and t.dim() == 3 and tuple(t.shape[1:]) == (kv, hd) and (t.stride(2) == 1 or t.numel() == 0), what,
+              f"k and v must be bf16 [rows, {kv}, {hd}], the channels contiguous")
+    _need(k.shape[0] == v.shape[0], what, "k and v differ in rows")
+    _lens(what, k.shape[0], slots=slots)
+    _need(all(_apart(t, c) for t in (k, v, slots) for c in cache), what, "an input lies in the cache")
+    _one_device(what, k, v, cache.codes, cache.scales, slots)
+    p = _lib.Kv4AppendParams()
+    p.k, p.v, p.codes, p.scales, p.slots = _p(k), _p(v), _p(cache.codes), _p(cache.scales), _p(slots)
+    p.sk_row, p.sk_head, p.sv_row, p.sv_head = k.stride(0), k.stride(1), v.stride(0), v.stride(1)
+    p.rows, p.kv, p.hd, p.page, p.pages = k.shape[0], kv, hd, P, pages
+    _lib.check(_lib.lib().grove_kv4_append(C.byref(p), _stream()), "grove_kv4_append")
+
+
+def kv4_read(cache, slots, out_dtype=bf16):
+    """(k, v) [rows, kv, hd], bf16 or f32: the values that the cache rows `slots` stand for; a slot outside the cache reads as zeros (grove_kv4_read)."""
+    what = "kv4_read"
+    pages, kv, P, hd = _kv4_shape(what, cache)
+    _need(out_dtype in (bf16, torch.float32), what, "out_dtype must be bf16 or f32")
+    _lens(what, slots.numel(), slots=slots)
+    _one_device(what, cache.codes, cache.scales, slots)
+    k, v = (torch.empty((slots.shape[0], kv, hd), dtype=out_dtype, device=slots.device) for _ in range(2))
+    p = _lib.Kv4ReadParams()
+    p.codes, p.scales, p.slots, p.k, p.v = _p(cache.codes), _p(cache.scales), _p(slots), _p(k), _p(v)
+    p.rows, p.kv, p.hd, p.page, p.pages, p.f32 = slots.shape[0], kv, hd, P, pages, int(out_dtype == torch.float32)
+    _lib.check(_lib.lib().grove_kv4_read(C.byref(p), _stream()), "grove_kv4_read")
+    return k, v
+
+
+def kv4_attn(q, cache, table, kv_len, cu_q, max_q, alpha, *, max_len=None, out=None):
+    """Causal attention of every request's new tokens over its 4-bit pages (grove_kv4_attn). q: bf16 [rows, heads, hd], any row and head strides;
+    table int32 [requests, max_pages]; kv_len int32 [requests] keys including the new tokens; cu_q int32 [requests + 1] (page_tables makes both);
+    max_q: the most new tokens that any request has. max_len: the longest kv_len if the host knows it (default: what the table holds); only the
+    split of the work goes by it. Returns bf16 [rows, heads * hd]; rows of no request are zero in a new tensor and stay as they were in `out`."""
+    what = "kv4_attn"
+    pages, kv, P, hd = _kv4_shape(what, cache)
+    _need(q.dtype == bf16 and q.dim() == 3 and q.shape[2] == hd and q.shape[1] % kv == 0 and q.shape[1] > 0, what, f"q must be bf16 [rows, a multiple of {kv}, {hd}]")
+    _need(q.stride(2) == 1 or q.numel() == 0, what, "the channels must be contiguous")
+    _need(table.dim() == 2 and table.dtype == torch.int32 and table.shape[0] > 0 and table.shape[1] > 0 and table.stride(1) == 1, what,
+          "table must be int32 [requests, max_pages], its rows contiguous")
+    B, rows, heads = table.shape[0], q.shape[0], q.shape[1]
+    _lens(what, B, kv_len=kv_len)
+    _lens(what, B + 1, cu_q=cu_q)
+    _need(B <= 65535 and max_q >= 0, what, "at most 65535 requests, max_q must not be negative")
+    _need(table.shape[1] * P < 2 ** 31, what, "the table holds more than 2^31 tokens")
+    if out is None:
+        _chk_dev(q)
+        out = torch.zeros((rows, heads * hd), dtype=bf16, device=q.device)
+    else:
+        _need(out.dtype == bf16 and tuple(out.shape) == (rows, heads * hd) and (out.stride(1) == 1 or out.numel() == 0) and _own_elements(out), what,
+              f"out must be bf16 [{rows}, {heads * hd}], its rows contiguous and apart")
+        _need(all(_apart(out, t) for t in (q, cache.codes, cache.scales, table, kv_len, cu_q)), what, "out overlaps an input")
+    _one_device(what, q, cache.codes, cache.scales, table, kv_len, cu_q, out)
+    p = _lib.Kv4AttnParams()
+    p.q, p.codes, p.scales, p.table, p.kv_len, p.cu_q, p.out = (_p(t) for t in (q, cache.codes, cache.scales, table, kv_len, cu_q, out))
+    p.sq_row, p.sq_head, p.so_row, p.ld_table = q.stride(0), q.stride(1), out.stride(0), max(table.stride(0), table.shape[1])
+    p.requests, p.heads, p.kv, p.hd, p.page, p.pages, p.max_pages = B, heads, kv, hd, P, pages, table.shape[1]
+    p.rows, p.max_q, p.n_split, p.alpha = rows, max_q, 1, float(alpha)
+    _lib.check(_lib.lib().grove_kv4_attn(C.byref(p), _stream()), "grove_kv4_attn")
+    return out
+
+
+def verify_drafts(draft, q, p, u, pick, count=None):
+    """(tokens int32 [requests, drafts + 1], accepted int32 [requests]): the drafts that the rejection rule accepts and the token after them, -1
+    behind (grove_verify_drafts). draft int32 [requests, drafts]; q f32 or bf16 [requests, drafts, vocab] the drafter's probabilities, None for a
+    drafter that is certain of its token; p [requests, drafts + 1, vocab] the target's, of the same type; u f32 [requests, drafts] and pick f32
+    [requests] uniform numbers of [0, 1); count int32 [requests]: drafts that a request has (default: all)."""
+    what = "verify_drafts"
+    _need(draft.dtype == torch.int32 and draft.dim() == 2 and draft.is_contiguous(), what, "draft must be contiguous int32 [requests, drafts]")
+    B, K = draft.shape
+    _need(p.dtype in (bf16, torch.float32) and p.dim() == 3 and tuple(p.shape[:2]) == (B, K + 1) and p.shape[2] > 0 and p.stride(2) == 1, what,
+          f"p must be f32 or bf16 [{B}, {K + 1}, vocab], its rows contiguous")
+    V = p.shape[2]
+    if K == 0:
+        q = None
+    _need(q is None or (q.dtype == p.dtype and tuple(q.shape) == (B, K, V) and q.stride(2) == 1), what, f"q must have p's type and be [{B}, {K}, {V}], its rows contiguous")
+    _need(u.dtype == torch.float32 and tuple(u.shape) == (B, K) and u.is_contiguous(), what, f"u must be contiguous f32 [{B}, {K}]")
+    _need(pick.dtype == torch.float32 and tuple(pick.shape) == (B,) and pick.is_contiguous(), what, f"pick must be contiguous f32 [{B}]")
+    if count is not None:
+        _lens(what, B, count=count)
+    _one_device(what, draft, q, p, u, pick, count)
+    tokens = torch.empty((B, K + 1), dtype=torch.int32, device=p.device)
+    accepted = torch.empty(B, dtype=torch.int32, device=p.device)
+    a = _lib.VerifyDraftsParams()
+    a.draft, a.q, a.p, a.u, a.pick, a.count, a.tokens, a.accepted = (_p(t) for t in (draft, q, p, u, pick, count, tokens, accepted))
+    a.sp_req, a.sp_row = p.stride(0), p.stride(1)
+    if q is not None:
+        a.sq_req, a.sq_row = q.stride(0), q.stride(1)
+    a.requests, a.drafts, a.vocab, a.bf16 = B, K, V, int(p.dtype == bf16)
+    _lib.check(_lib.lib().grove_verify_drafts(C.byref(a), _stream()), "grove_verify_drafts")
+    return tokens, accepted

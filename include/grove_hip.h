@@ -618,6 +618,138 @@ typedef struct grove_greedy_pick_params {
 int grove_greedy_pick(const grove_greedy_pick_params* p, void* stream);
 
 /* ------------------------------------------------------------------------------------------
+ * Serving from a paged 4-bit key / value cache with drafted tokens: what the cached decode step (grove_decode_attn,
+ * grove_greedy_pick) becomes when requests of unlike lengths share one pool of pages and a step carries several tokens per
+ * request. One step: page_tables -> rotary -> kv4_append -> kv4_attn -> verify_drafts.
+ *
+ * The rows of a step (its new tokens) are packed request after request: request b owns rows cu_q[b] .. cu_q[b + 1] - 1.
+ * A page holds `page` (16, 32, 64, 128 or 256) consecutive tokens of one request for every key / value head; token t of request
+ * b lies in page table[b, t / page] at offset t % page, its slot is page * page_size + offset.
+ * ------------------------------------------------------------------------------------------ */
+
+/* Rotary positions of rows x heads x hd, fp32 arithmetic, in place (y == x, same strides) or into y:
+ *   pair i of a head, i < rot / 2, is (x[i], x[i + rot / 2]) (interleaved = 0) or (x[2 i], x[2 i + 1]) (interleaved = 1) and becomes
+ *   mscale * (a cos t - b sin t, b cos t + a sin t) with t = pos[row] * freq[i]; channels >= rot pass through.
+ * backward = 1: the transpose (sin -> -sin), which is the gradient w.r.t. x for the gradient w.r.t. y.
+ * The angle is formed and reduced to a part of a turn in fp64, so positions of millions keep fp32 accuracy. */
+typedef struct grove_rotary_params {
+  const void* x; /* bf16, or f32 if `f32` */
+  void* y;
+  const int32_t* pos; /* [rows] */
+  const double* freq; /* [rot / 2] radians per position */
+  int64_t sx_row, sx_head, sy_row, sy_head; /* strides in elements; channels are contiguous */
+  int32_t rows, heads, hd, rot;
+  int32_t interleaved, backward, f32;
+  float mscale;
+} grove_rotary_params;
+int grove_rotary(const grove_rotary_params* p, void* stream);
+
+/* The tables of one step from the requests' lengths, on the device. Per request b (negative lengths count as 0):
+ *   kv_len[b] = ctx_len[b] + new_len[b]; need = max(0, min(ceil(kv_len / page), max_pages) - held[b]);
+ *   table[b, held[b] + i] = free_pages[start_b + i] for i < need, start_b = the needs of the requests before b (in place; the
+ *   other entries stay); held_out[b] = held[b] + the pages that b got. Where the free list is too short the entry is -1, and *taken, the
+ *   sum of the needs, says so: taken > n_free.
+ *   cu_q[b] = the new tokens of the requests before b; cu_q[requests] = all.
+ * Per row r of the step: pos[r] = ctx_len[b] + (r - cu_q[b]), slots[r] = its slot, -1 where its page is missing. Rows
+ * cu_q[requests] .. rows - 1 get slot -1 and position 0 (a captured step of fixed size); rows past `rows` are not written.
+ * requests is at most 4096. held_out may not be held, nor kv_len ctx_len or new_len. */
+typedef struct grove_page_tables_params {
+  const int32_t* ctx_len;    /* [requests] */
+  const int32_t* new_len;    /* [requests] */
+  const int32_t* held;       /* [requests] pages a request has */
+  const int32_t* free_pages; /* [n_free] */
+  int32_t* table;            /* [requests, ld_table] */
+  int32_t* kv_len;           /* [requests] out */
+  int32_t* cu_q;             /* [requests + 1] out */
+  int32_t* slots;            /* [rows] out */
+  int32_t* pos;              /* [rows] out */
+  int32_t* held_out;         /* [requests] out */
+  int32_t* taken;            /* [1] out */
+  int64_t ld_table;
+  int32_t requests, max_pages, page, rows, n_free;
+} grove_page_tables_params;
+int grove_page_tables(const grove_page_tables_params* p, void* stream);
+
+/* The 4-bit cache. A row (one token, one head, hd channels; hd 32, 64, 128 or 256) is held as hd codes c in 0..15, a scale s and a
+ * minimum m, both bf16, and stands for m + c s:
+ *   m = min(row), s = bf16((max - min) / 15), c = clamp(rint((x - m) / s), 0, 15)    (s = 0 and c = 0 where max - min < 2^-100).
+ * A row that holds an infinity or a NaN, or whose range passes fp32, is held as NaN as a whole.
+ *   codes:  uint8 [pages, 2, kv, page * hd / 2]   keys, values
+ *   scales: bf16  [pages, 2, kv, page, 2]         (s, m)
+ * Order of the codes, made for the attention kernel's matrix operands. Keys: a row is 4 pieces h of hd / 32 words (32 bits); word t of
+ * piece h holds channels 32 t + 8 h + {0, 2, 4, 6, 1, 3, 5, 7}, lowest nibble first. Values: four tokens together; for each m of
+ * 0..15, the channels 16 j + m of the four: 16 bits of four j per token, in the order (j block, token); hd = 32, with its two j: 8 bits
+ * per token, tokens in the order 0, 2, 1, 3. */
+
+/* Quantises rows of k and v into the cache rows of `slots`; a slot outside [0, pages * page) is skipped. The slots that are kept
+ * are distinct (those of grove_page_tables are): two rows of one slot would leave a mixture of both. */
+typedef struct grove_kv4_append_params {
+  const void* k; /* bf16 [rows, kv, hd], strides below, channels contiguous */
+  const void* v;
+  void* codes;
+  void* scales;
+  const int32_t* slots; /* [rows] */
+  int64_t sk_row, sk_head, sv_row, sv_head;
+  int32_t rows, kv, hd, page, pages;
+} grove_kv4_append_params;
+int grove_kv4_append(const grove_kv4_append_params* p, void* stream);
+
+/* The values that the cache rows of `slots` stand for (fp32, rounded once where the output is bf16); a slot outside reads as zeros. */
+typedef struct grove_kv4_read_params {
+  const void* codes;
+  const void* scales;
+  const int32_t* slots; /* [rows] */
+  void* k;              /* bf16 or f32 [rows, kv, hd] contiguous, out */
+  void* v;
+  int32_t rows, kv, hd, page, pages, f32;
+} grove_kv4_read_params;
+int grove_kv4_read(const grove_kv4_read_params* p, void* stream);
+
+/* Causal attention of the new tokens of every request over its pages (its own rows appended before). q: bf16 [rows, heads, hd],
+ * query head j reads key / value head j / (heads / kv); out: bf16 [rows, heads * hd].
+ *   row r = cu_q[b] + i of request b with n = cu_q[b + 1] - cu_q[b] new tokens sees the keys t < kv_len[b] - n + i + 1:
+ *   out[r] = softmax(alpha * q[r] . K[t]) V, fp32 throughout; 0 where it sees none.
+ * Keys whose table entry is outside [0, pages) are not seen. kv_len is cut to max_pages * page. Rows of no request are left as they
+ * were. n must not pass max_q. Rows of the cache that no query sees may hold anything.
+ * n_split > 1: a request's keys are dealt to n_split blocks, whose partial results lie in `partial`, f32 [rows * heads * n_split *
+ * (hd + 2)], and are joined by a second launch. Otherwise `partial` may be NULL. */
+typedef struct grove_kv4_attn_params {
+  const void* q;
+  const void* codes;
+  const void* scales;
+  const int32_t* table;  /* [requests, ld_table] */
+  const int32_t* kv_len; /* [requests] */
+  const int32_t* cu_q;   /* [requests + 1] */
+  void* out;
+  float* partial;
+  int64_t sq_row, sq_head, so_row, ld_table;
+  int32_t requests, heads, kv, hd, page, pages, max_pages, rows, max_q, n_split;
+  float alpha;
+} grove_kv4_attn_params;
+int grove_kv4_attn(const grove_kv4_attn_params* p, void* stream);
+
+/* Verification of drafted tokens by the rejection rule that leaves the target's distribution unchanged. Request b has
+ * n = count[b] drafts (count NULL: all `drafts`; cut to 0..drafts). Draft i is accepted while u[b, i] * q[b, i, x_i] < p[b, i, x_i];
+ * accepted[b] = a = the drafts before the first refused one. The token after them is the smallest t with
+ *   sum_{j <= t} r[j] > pick[b] * sum_j r[j],   r = max(p[b, a] - q[b, a], 0) where draft a was refused, p[b, n] where none was
+ * (p itself too where the difference leaves nothing; the last t with r > 0 where rounding leaves no such t; -1 where p holds nothing).
+ * tokens[b] = the accepted drafts, that token, then -1. q NULL: a drafter that is certain of its token (q = 1 at x_i, 0 elsewhere).
+ * Products, differences and sums are fp64. A draft outside [0, vocab) is refused. u and pick lie in [0, 1). */
+typedef struct grove_verify_drafts_params {
+  const int32_t* draft; /* [requests, drafts] contiguous */
+  const void* q;        /* f32 or bf16 [requests, drafts, vocab] */
+  const void* p;        /* f32 or bf16 [requests, drafts + 1, vocab] */
+  const float* u;       /* [requests, drafts] contiguous */
+  const float* pick;    /* [requests] */
+  const int32_t* count; /* [requests] or NULL */
+  int32_t* tokens;      /* [requests, drafts + 1] out */
+  int32_t* accepted;    /* [requests] out */
+  int64_t sq_req, sq_row, sp_req, sp_row;
+  int32_t requests, drafts, vocab, bf16;
+} grove_verify_drafts_params;
+int grove_verify_drafts(const grove_verify_drafts_params* p, void* stream);
+
+/* ------------------------------------------------------------------------------------------
  * Frame preprocessing on the device. One separable pass of Pillow's 8-bit resampler
  * (ImagingResample: 22-bit fixed-point coefficients, half-up rounding, uint8 clamp) over uint8 RGB frames
  * [F, H, W, 3]; the reference runs it on the host through torchvision / transformers:
