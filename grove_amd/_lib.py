@@ -191,7 +191,7 @@ class Kv4AttnParams(C.Structure):
     _fields_ = [("q", c_vp), ("codes", c_vp), ("scales", c_vp), ("table", c_vp), ("kv_len", c_vp), ("cu_q", c_vp), ("out", c_vp), ("partial", c_vp),
                 ("sq_row", c_i64), ("sq_head", c_i64), ("so_row", c_i64), ("ld_table", c_i64),
                 ("requests", c_i32), ("heads", c_i32), ("kv", c_i32), ("hd", c_i32), ("page", c_i32), ("pages", c_i32), ("max_pages", c_i32),
-                ("rows", c_i32), ("max_q", c_i32), ("n_split", c_i32), ("alpha", c_f32)]
+                ("rows", c_i32), ("max_q", c_i32), ("n_split", c_i32), ("fresh", c_i32), ("alpha", c_f32)]
 
 
 class VerifyDraftsParams(C.Structure):

@@ -1,5 +1,6 @@
 // The paged 4-bit key / value cache (layout: grove_hip.h): quantise into pages, read back, attend.
 #include "common.h"
+#include <type_traits>
 
 namespace {
 
@@ -82,64 +83,342 @@ __global__ __launch_bounds__(64) void kv4_read_kernel(const grove_kv4_read_param
   }
 }
 
-// One wave per (row, query head): 64 keys at a time, a lane each for the scores; then a lane per channel for the values.
+// ---------------------------------------------------------------- attention over 4-bit pages
+// A block of four waves takes one (request, key / value head, range of keys) and up to 16 CT query columns: the group's query heads of the
+// request's new tokens side by side (column = token * group + head). 32 keys at a time and wave, from two 16-key parts of a page:
+//   S^T[key, col] = sum_c K[key, c] q[col, c]   A = keys (16) x 32 channels, B = columns: the codes go to the matrix unit as bf16 16 + c, which a
+//     shift and one and-or make of a nibble pair (exact; the offset is taken off with the row's minimum), so a key costs no multiply for its scale:
+//     z = (alpha' s) raw + (m - 16 s) (alpha' sum q), in units of log2.
+//   O^T[c, col] += sum_key V[key, c] (P s)[key, col]   A = channels (16) x 32 keys, B = the scores' own registers: the accumulator of S^T holds keys
+//     4 h + i of either part in lane (col, h), and the values' four-token order gives the A operand the same keys. P s goes in as two bf16 parts
+//     (hi + lo, 2^-17), the minimum's share sum P (m - 16 s) is one number per column.
+// Running maximum in log2 units, raised only where a score passes it by 8 (P <= 2^8 keeps its precision in fp32): most tiles skip the rescaling.
 template <int HD>
-__global__ __launch_bounds__(64) void kv4_attn_simple_kernel(const grove_kv4_attn_params p) {
-  __shared__ float q[HD], pr[64];
-  __shared__ int pages[64];
-  const int lane = threadIdx.x, row = blockIdx.x, head = blockIdx.y, kvh = head / (p.heads / p.kv);
-  int b = -1;
-  for (int i = 0; i < p.requests; ++i)
-    if (row >= p.cu_q[i] && row < p.cu_q[i + 1]) b = i;
-  if (b < 0) return;
-  const int n = p.cu_q[b + 1] - p.cu_q[b], len = p.kv_len[b];
-  const int64_t room = (int64_t)p.max_pages * p.page;
-  const int seen = (int)min(room, (int64_t)len - n + (row - p.cu_q[b]) + 1);
-  const bf16_raw* x = (const bf16_raw*)p.q + row * p.sq_row + head * p.sq_head;
-  for (int c = lane; c < HD; c += 64) q[c] = bf2f(x[c]);
-  constexpr int NC = (HD + 63) / 64;
-  float acc[NC] = {}, mx = -INFINITY, sum = 0.f;
-  for (int t0 = 0; t0 < seen; t0 += 64) {
-    __syncthreads();
-    const int t = t0 + lane;
-    const int pg = t < seen ? p.table[b * p.ld_table + t / p.page] : -1;
-    pages[lane] = pg;
-    float z = -INFINITY;
-    if (pg >= 0 && pg < p.pages) {
-      const int64_t plane = (int64_t)pg * 2 * p.kv + kvh;
-      const unsigned char* in = (const unsigned char*)p.codes + plane * p.page * (HD / 2);
-      const unsigned sm = ((const unsigned*)p.scales)[plane * p.page + t % p.page];
-      z = 0.f;
-      for (int c = 0; c < HD; ++c) {
-        int up;
-        const int byte = key_byte<HD>(t % p.page, c, up);
-        z = fmaf(q[c], fmaf((float)((in[byte] >> (4 * up)) & 15), bf_lo(sm), bf_hi(sm)), z);
-      }
-      z *= p.alpha;
+struct kv4_tile {
+  unsigned k[2][HD / 32], v[2][HD / 32];
+  u32x4_t ks[2], vs[2];
+  int page[2];  // -1: not a page of the cache
+};
+
+template <int N>
+__device__ __forceinline__ void ld_words(unsigned* d, const unsigned char* a) {
+  if constexpr (N == 1) d[0] = *(const unsigned*)a;
+  else if constexpr (N == 2) { const u32x2_t x = *(const u32x2_t*)a; d[0] = x[0]; d[1] = x[1]; }
+  else
+#pragma unroll
+    for (int i = 0; i < N; i += 4) {
+      const u32x4_t x = *(const u32x4_t*)(a + 4 * i);
+      d[i] = x[0]; d[i + 1] = x[1]; d[i + 2] = x[2]; d[i + 3] = x[3];
     }
-    const float top = fmaxf(mx, wave_max(z)), ref = top == -INFINITY ? 0.f : top;
-    const float e = z == -INFINITY ? 0.f : expf(z - ref), keep = mx == -INFINITY ? 0.f : expf(mx - ref);
-    mx = top;
-    sum = sum * keep + wave_sum(e);
-    pr[lane] = e;
-    __syncthreads();
-    for (int i = 0; i < NC; ++i) acc[i] *= keep;
-    for (int k = 0; k < 64; ++k) {
-      const int pk = pages[k];
-      if (pk < 0 || pk >= p.pages) continue;
-      const int64_t plane = ((int64_t)pk * 2 + 1) * p.kv + kvh;
-      const unsigned char* in = (const unsigned char*)p.codes + plane * p.page * (HD / 2);
-      const int at = (t0 + k) % p.page;
-      const unsigned sm = ((const unsigned*)p.scales)[plane * p.page + at];
-      for (int i = 0, c = lane; c < HD; c += 64, ++i) {
-        int up;
-        const int byte = value_byte<HD>(at, c, up);
-        acc[i] = fmaf(pr[k], fmaf((float)((in[byte] >> (4 * up)) & 15), bf_lo(sm), bf_hi(sm)), acc[i]);
-      }
+}
+
+// Nibble j of either half of a word as a pair of bf16 16 + c: the nibble on mantissa bits 3..6 below the exponent of 16.
+__device__ __forceinline__ unsigned code_pair(unsigned w, int j) {
+  const unsigned x = j == 0 ? w << 3 : w >> (4 * j - 3);
+  return (x & 0x00780078u) | 0x41804180u;
+}
+__device__ __forceinline__ bf16x8_t frag(unsigned a, unsigned b, unsigned c, unsigned d) { return __builtin_bit_cast(bf16x8_t, (u32x4_t){a, b, c, d}); }
+
+constexpr float NEG = -INFINITY;
+
+constexpr int KV4_WAVES(int hd, int ct) { return hd * ct <= 128 ? 2 : 1; }
+
+template <int HD, int CT>
+__global__ __launch_bounds__(256, KV4_WAVES(HD, CT)) void kv4_attn_kernel(const grove_kv4_attn_params p, const int shift, const int vec_q, const int vec_o) {
+  constexpr int NK = HD / 32, NJ = HD / 16, HC = HD < 128 ? HD : 128;  // HC channels go through LDS at a time
+  __shared__ float s_m[4][16 * CT], s_l[4][16 * CT], s_c[4][16 * CT];
+  __shared__ float s_o[4][16][HC + 4];
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), n16 = lane & 15, h = lane >> 4;
+  const int G = p.heads / p.kv, chunks = gridDim.y / p.kv, hk = blockIdx.y / chunks, cc = blockIdx.y - hk * chunks, b = blockIdx.z, sp = blockIdx.x;
+  if (p.fresh && p.n_split == 1 && b == 0 && cc == 0) {  // a new result's rows of no request
+    const int r0 = max(0, min(p.cu_q[0], p.rows)), r1 = max(r0, min(p.cu_q[p.requests], p.rows));
+    for (int64_t e = tid; e < (int64_t)(r0 + p.rows - r1) * G * HD; e += 256) {
+      const int r = (int)(e / (G * HD));
+      ((bf16_raw*)p.out)[(r < r0 ? r : r1 + r - r0) * p.so_row + (int64_t)hk * G * HD + e % (G * HD)] = 0;
     }
   }
+  const int t0 = max(0, min(p.cu_q[b], p.rows)), t1 = max(t0, min(p.cu_q[b + 1], p.rows)), n = t1 - t0;
+  const int cols = min(n, p.max_q) * G, col0 = cc * 16 * CT;
+  if (col0 >= cols) return;
+  const int64_t room = (int64_t)p.max_pages << shift;
+  const int base = (int)min((int64_t)p.kv_len[b], room) - n + 1;  // token i sees base + i keys
+  const int seen_all = max(0, base + col0 / G), seen_any = max(0, base + (min(cols, col0 + 16 * CT) - 1) / G);
+  const int tiles = (seen_any + 31) >> 5, per = (tiles + p.n_split - 1) / p.n_split, tile0 = sp * per, tile1 = min(tiles, tile0 + per);
+
+  bf16x8_t q[CT][NK];
+  float qs[CT], m[CT], l[CT], cst[CT];
+  int lim[CT];
+  const float a2 = p.alpha * 1.44269504088896340736f;
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) {
+    const int c = col0 + ct * 16 + n16, i = c / G;
+    const bf16_raw* x = (const bf16_raw*)p.q + (t0 + i) * p.sq_row + (int64_t)(hk * G + c - i * G) * p.sq_head + 8 * h;
+    float sum = 0.f;
+#pragma unroll
+    for (int t = 0; t < NK; ++t) {
+      u32x4_t r = {0, 0, 0, 0};
+      if (c < cols) {
+        if (vec_q) r = *(const u32x4_t*)(x + 32 * t);
+        else
+          for (int e = 0; e < 4; ++e) r[e] = x[32 * t + 2 * e] | ((unsigned)x[32 * t + 2 * e + 1] << 16);
+      }
+      q[ct][t] = __builtin_bit_cast(bf16x8_t, r);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sum += bf_lo(r[e]) + bf_hi(r[e]);
+    }
+    sum += __shfl_xor(sum, 16, 64);
+    sum += __shfl_xor(sum, 32, 64);
+    qs[ct] = sum * a2;
+    lim[ct] = c < cols ? base + i : 0;
+    m[ct] = NEG;
+    l[ct] = cst[ct] = 0.f;
+  }
+  f32x4_t acc[CT][NJ];
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) acc[ct][j] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
+
+  // page numbers: 64 of them in the lanes, refilled when the wave has passed them
+  const int* row = p.table + b * p.ld_table;
+  int pg_lo = 0, pg_lane = -1;
+  bool have = false;
+  auto page_of = [&](int pi) -> int {  // pi: the same in all lanes, never below an earlier one
+    if (!have || pi >= pg_lo + 64) {
+      pg_lo = pi;
+      pg_lane = pi + lane < p.max_pages ? row[pi + lane] : -1;
+      have = true;
+    }
+    const int pg = __builtin_amdgcn_readlane(pg_lane, pi - pg_lo);
+    return pg >= 0 && pg < p.pages ? pg : -1;
+  };
+  const int P = 1 << shift;
+  auto load = [&](int tile, kv4_tile<HD>& T) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int t = tile * 32 + 16 * u, pg = page_of(t >> shift), r = t & (P - 1);
+      T.page[u] = pg;
+      const int64_t plane = ((int64_t)max(pg, 0) * 2) * p.kv + hk;  // a missing page's keys are masked; its loads go to page 0
+      const unsigned char* kc = (const unsigned char*)p.codes + (plane << shift) * (HD / 2) + r * (HD / 2);
+      const unsigned char* vc = kc + ((int64_t)p.kv << shift) * (HD / 2);
+      ld_words<NK>(T.k[u], kc + n16 * (HD / 2) + h * (HD / 8));
+      ld_words<NK>(T.v[u], vc + h * (2 * HD) + n16 * (HD / 8));
+      const unsigned* sc = (const unsigned*)p.scales + (plane << shift) + r + 4 * h;
+      T.ks[u] = *(const u32x4_t*)sc;
+      T.vs[u] = *(const u32x4_t*)(sc + ((int64_t)p.kv << shift));
+    }
+  };
+  auto compute = [&](int tile, const kv4_tile<HD>& T, auto masked) {
+    constexpr bool MASK = decltype(masked)::value;
+    float z[CT][8];
+    auto sees = [&](int ct, int u, int i) { return tile * 32 + 16 * u + 4 * h + i < lim[ct] && T.page[u] >= 0; };
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      __builtin_amdgcn_sched_barrier(0);  // one part's operands at a time: unpacked all at once they would take the registers of a third wave
+      bf16x8_t kf[NK];
+#pragma unroll
+      for (int t = 0; t < NK; ++t) kf[t] = frag(code_pair(T.k[u][t], 0), code_pair(T.k[u][t], 1), code_pair(T.k[u][t], 2), code_pair(T.k[u][t], 3));
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) {
+        f32x4_t raw = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int t = 0; t < NK; ++t) raw = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[t], q[ct][t], raw, 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float s = bf_lo(T.ks[u][i]), mn = bf_hi(T.ks[u][i]);
+          float v = fmaf(raw[i], a2 * s, fmaf(-16.f, s, mn) * qs[ct]);
+          if constexpr (MASK) v = sees(ct, u, i) ? v : NEG;
+          z[ct][4 * u + i] = v;
+        }
+      }
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    float top[CT];
+    bool grow = false;
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+      top[ct] = z[ct][0];
+#pragma unroll
+      for (int i = 1; i < 8; ++i) top[ct] = fmaxf(top[ct], z[ct][i]);
+      grow |= top[ct] > m[ct] + 8.f;
+    }
+    if (__any(grow)) {
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) {
+        float t = fmaxf(top[ct], __shfl_xor(top[ct], 16, 64));
+        t = fmaxf(t, __shfl_xor(t, 32, 64));
+        t = fmaxf(t, m[ct]);
+        const float f = m[ct] == NEG ? 0.f : __builtin_amdgcn_exp2f(m[ct] - t);
+        m[ct] = t;
+        l[ct] *= f;
+        cst[ct] *= f;
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) acc[ct][j] *= f;
+      }
+    }
+    bf16x8_t hi[CT], lo[CT];
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+      const float ref = m[ct] == NEG ? 0.f : m[ct];
+      unsigned a[4], c[4];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        float ps[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float e = __builtin_amdgcn_exp2f(z[ct][4 * u + i] - ref);
+          const float s = bf_lo(T.vs[u][i]), mn = fmaf(-16.f, s, bf_hi(T.vs[u][i]));
+          l[ct] += e;
+          ps[i] = e * s;
+          float pm = e * mn;
+          if constexpr (MASK) {  // an unseen row's scale may be anything
+            ps[i] = sees(ct, u, i) ? ps[i] : 0.f;
+            pm = sees(ct, u, i) ? pm : 0.f;
+          }
+          cst[ct] += pm;
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          a[2 * u + i] = pack2bf(ps[2 * i], ps[2 * i + 1]);
+          c[2 * u + i] = pack2bf(ps[2 * i] - bf_lo(a[2 * u + i]), ps[2 * i + 1] - bf_hi(a[2 * u + i]));
+        }
+      }
+      hi[ct] = frag(a[0], a[1], a[2], a[3]);
+      lo[ct] = frag(c[0], c[1], c[2], c[3]);
+    }
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) {
+      if ((j & 1) == 0) __builtin_amdgcn_sched_barrier(0);
+      bf16x8_t vf;
+      if constexpr (HD == 32) vf = frag(code_pair(T.v[0][0], j), code_pair(T.v[0][0], j + 2), code_pair(T.v[1][0], j), code_pair(T.v[1][0], j + 2));
+      else {
+        const int o = (j >> 2) * 2, jn = j & 3;
+        vf = frag(code_pair(T.v[0][o], jn), code_pair(T.v[0][o + 1], jn), code_pair(T.v[1][o], jn), code_pair(T.v[1][o + 1], jn));
+      }
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) {
+        acc[ct][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, hi[ct], acc[ct][j], 0, 0, 0);
+        acc[ct][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, lo[ct], acc[ct][j], 0, 0, 0);
+      }
+    }
+  };
+
+  int tile = tile0 + w;
+  if (tile < tile1) {
+    kv4_tile<HD> cur, nxt;
+    load(tile, cur);
+    while (true) {
+      const int next = tile + 4;
+      if (next < tile1) load(next, nxt);
+      if ((tile + 1) * 32 <= seen_all && cur.page[0] >= 0 && cur.page[1] >= 0) compute(tile, cur, std::false_type{});
+      else compute(tile, cur, std::true_type{});
+      if (next >= tile1) break;
+      cur = nxt;
+      tile = next;
+    }
+  }
+
+  // the four waves' results: one maximum per column, the outputs through LDS
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) {
+    l[ct] += __shfl_xor(l[ct], 16, 64);
+    l[ct] += __shfl_xor(l[ct], 32, 64);
+    cst[ct] += __shfl_xor(cst[ct], 16, 64);
+    cst[ct] += __shfl_xor(cst[ct], 32, 64);
+    if (h == 0) {
+      s_m[w][ct * 16 + n16] = m[ct];
+      s_l[w][ct * 16 + n16] = l[ct];
+      s_c[w][ct * 16 + n16] = cst[ct];
+    }
+  }
+  __syncthreads();
+  const bool split = p.n_split > 1;
+  const int oc = tid >> 4, och = (tid & 15) * (HC / 16);
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) {
+    auto joint = [&](int col) { return fmaxf(fmaxf(s_m[0][col], s_m[1][col]), fmaxf(s_m[2][col], s_m[3][col])); };
+    auto part = [&](float mw, float M) { return mw == NEG ? 0.f : __builtin_amdgcn_exp2f(mw - M); };
+    const float f = part(m[ct], joint(ct * 16 + n16));
+    const int col = ct * 16 + oc, c = col0 + col, i = c / G;
+    const float M = joint(col);
+    float L = 0.f, C = 0.f;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float fk = part(s_m[k][col], M);
+      L += fk * s_l[k][col];
+      C += fk * s_c[k][col];
+    }
+    const int64_t unit = (int64_t)(t0 + i) * p.heads + hk * G + (c - i * G);
+    if (split && c < cols && (tid & 15) == 0) {
+      float* ml = p.partial + (int64_t)p.rows * p.heads * p.n_split * HD + (unit * p.n_split + sp) * 2;
+      ml[0] = M;
+      ml[1] = L;
+    }
+#pragma unroll
+    for (int c0 = 0; c0 < HD; c0 += HC) {
+#pragma unroll
+      for (int j = 0; j < HC / 16; ++j) *(f32x4_t*)&s_o[w][n16][16 * j + 4 * h] = acc[ct][c0 / 16 + j] * f;
+      __syncthreads();
+      if (c < cols) {
+        float o[HC / 16];
+#pragma unroll
+        for (int e = 0; e < HC / 16; ++e) o[e] = C + ((s_o[0][oc][och + e] + s_o[1][oc][och + e]) + (s_o[2][oc][och + e] + s_o[3][oc][och + e]));
+        if (split) {
+          float* y = p.partial + (unit * p.n_split + sp) * HD + c0 + och;
+#pragma unroll
+          for (int e = 0; e < HC / 16; ++e) y[e] = o[e];
+        } else {
+          bf16_raw* y = (bf16_raw*)p.out + (t0 + i) * p.so_row + (int64_t)(hk * G + c - i * G) * HD + c0 + och;
+          const float r = L > 0.f || L != L ? 1.f / L : 0.f;
+          unsigned pk[HC / 32];
+#pragma unroll
+          for (int e = 0; e < HC / 32; ++e) pk[e] = L > 0.f || L != L ? pack2bf(o[2 * e] * r, o[2 * e + 1] * r) : 0u;
+          if (vec_o) {
+#pragma unroll
+            for (int e = 0; e < HC / 32; ++e) ((unsigned*)y)[e] = pk[e];
+          } else {
+#pragma unroll
+            for (int e = 0; e < HC / 16; ++e) y[e] = (bf16_raw)(pk[e >> 1] >> (16 * (e & 1)));
+          }
+        }
+      }
+      __syncthreads();
+    }
+  }
+}
+
+// Joins the partial results of the splits: one wave per (row, query head).
+template <int HD>
+__global__ __launch_bounds__(256) void kv4_join_kernel(const grove_kv4_attn_params p) {
+  constexpr int NC = HD < 64 ? 1 : HD / 64;
+  const int lane = threadIdx.x & 63, S = p.n_split;
+  const int64_t unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (unit >= (int64_t)p.rows * p.heads) return;
+  const int row = (int)(unit / p.heads), head = (int)(unit - (int64_t)row * p.heads);
+  const bool mine = row >= p.cu_q[0] && row < p.cu_q[p.requests];
+  if (!mine && !p.fresh) return;
   bf16_raw* y = (bf16_raw*)p.out + row * p.so_row + (int64_t)head * HD;
-  for (int i = 0, c = lane; c < HD; c += 64, ++i) y[c] = f2bf(sum > 0.f || sum != sum ? acc[i] / sum : 0.f);
+  float o[NC] = {}, L = 0.f;
+  if (mine) {
+    const float* ml = p.partial + (int64_t)p.rows * p.heads * S * HD + unit * S * 2;
+    const float* part = p.partial + unit * S * HD;
+    float M = NEG;
+    for (int s = lane; s < S; s += 64) M = fmaxf(M, ml[2 * s]);
+    M = wave_max(M);
+    for (int s = 0; s < S; ++s) {
+      const float ms = ml[2 * s], ls = ml[2 * s + 1];
+      if (ls == 0.f) continue;  // a split without keys wrote no output
+      const float f = ms == NEG ? 0.f : __builtin_amdgcn_exp2f(ms - M);
+      L += f * ls;
+#pragma unroll
+      for (int i = 0; i < NC; ++i)
+        if (HD >= 64 || lane < HD) o[i] += f * part[(int64_t)s * HD + lane + 64 * i];
+    }
+  }
+  const bool some = L > 0.f || L != L;
+#pragma unroll
+  for (int i = 0; i < NC; ++i)
+    if (HD >= 64 || lane < HD) y[lane + 64 * i] = some ? f2bf(o[i] / L) : (bf16_raw)0;
 }
 
 bool page_ok(int page) { return page == 16 || page == 32 || page == 64 || page == 128 || page == 256; }
@@ -194,9 +473,30 @@ extern "C" int grove_kv4_attn(const grove_kv4_attn_params* p, void* stream) {
   if (p->rows == 0 || p->requests == 0 || p->max_q == 0) return GROVE_OK;
   GROVE_CHECK(p->q && p->codes && p->scales && p->table && p->kv_len && p->cu_q && p->out, GROVE_E_SHAPE, "kv4_attn: null pointer");
   GROVE_CHECK(((uintptr_t)p->codes & 15) == 0 && ((uintptr_t)p->scales & 15) == 0, GROVE_E_ALIGN, "kv4_attn: the cache must be 16-byte aligned");
-#define LAUNCH(HD) hipLaunchKernelGGL(kv4_attn_simple_kernel<HD>, dim3((unsigned)p->rows, (unsigned)p->heads), dim3(64), 0, (hipStream_t)stream, *p)
+  GROVE_CHECK(p->n_split >= 1 && p->n_split <= 65535 && (p->n_split == 1 || p->partial), GROVE_E_WORKSPACE, "kv4_attn: a split needs its workspace");
+  GROVE_CHECK((int64_t)p->max_pages * p->page <= 0x7fffffff, GROVE_E_SHAPE, "kv4_attn: the table holds more than 2^31 tokens");
+  const int shift = __builtin_ctz((unsigned)p->page);
+  const int vec_q = ((uintptr_t)p->q & 15) == 0 && p->sq_row % 8 == 0 && p->sq_head % 8 == 0, vec_o = ((uintptr_t)p->out & 15) == 0 && p->so_row % 8 == 0;
+  // columns that one pass over a key can serve: as few tiles of 16 as hold them, at most 64 (32 at hd 256, whose outputs fill the registers)
+  const int64_t cols = (int64_t)(p->max_q < p->rows ? p->max_q : p->rows) * (p->heads / p->kv);
+  const int ct = cols <= 16 ? 1 : cols <= 32 || p->hd == 256 ? 2 : 4;
+  const int64_t chunks = (cols + 16 * ct - 1) / (16 * ct);
+  GROVE_CHECK(chunks * p->kv <= 65535, GROVE_E_SHAPE, "kv4_attn: too many new tokens in a request (%lld columns)", (long long)cols);
+  const dim3 grid((unsigned)p->n_split, (unsigned)(chunks * p->kv), (unsigned)p->requests);
+#define LAUNCH(HD)                                                                                                                            \
+  if (ct == 1) hipLaunchKernelGGL((kv4_attn_kernel<HD, 1>), grid, dim3(256), 0, (hipStream_t)stream, *p, shift, vec_q, vec_o);                \
+  else if (ct == 2) hipLaunchKernelGGL((kv4_attn_kernel<HD, 2>), grid, dim3(256), 0, (hipStream_t)stream, *p, shift, vec_q, vec_o);           \
+  else hipLaunchKernelGGL((kv4_attn_kernel<HD < 256 ? HD : 128, 4>), grid, dim3(256), 0, (hipStream_t)stream, *p, shift, vec_q, vec_o)
   KV4_HD(p->hd, LAUNCH)
 #undef LAUNCH
   GROVE_LAUNCH_CHECK();
+  if (p->n_split > 1) {
+    const int64_t units = (int64_t)p->rows * p->heads;
+    GROVE_CHECK((units + 3) / 4 <= 0x7fffffff, GROVE_E_SHAPE, "kv4_attn: too many rows");
+#define LAUNCH(HD) hipLaunchKernelGGL(kv4_join_kernel<HD>, dim3((unsigned)((units + 3) / 4)), dim3(256), 0, (hipStream_t)stream, *p)
+    KV4_HD(p->hd, LAUNCH)
+#undef LAUNCH
+    GROVE_LAUNCH_CHECK();
+  }
   return GROVE_OK;
 }

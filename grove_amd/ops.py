@@ -1383,6 +1383,12 @@ def kv4_read(cache, slots, out_dtype=bf16):
     return k, v
 
 
+def _kv4_split(pairs, max_len, cols):
+    """Blocks to which a request's keys are dealt."""
+    blocks = pairs * max(1, -(-cols // 64))
+    return max(1, min(64, max_len // 512, 2048 // blocks))
+
+
 def kv4_attn(q, cache, table, kv_len, cu_q, max_q, alpha, *, max_len=None, out=None):
     """Causal attention of every request's new tokens over its 4-bit pages (grove_kv4_attn). q: bf16 [rows, heads, hd], any row and head strides;
     table int32 [requests, max_pages]; kv_len int32 [requests] keys including the new tokens; cu_q int32 [requests + 1] (page_tables makes both);
@@ -1399,9 +1405,10 @@ def kv4_attn(q, cache, table, kv_len, cu_q, max_q, alpha, *, max_len=None, out=N
     _lens(what, B + 1, cu_q=cu_q)
     _need(B <= 65535 and max_q >= 0, what, "at most 65535 requests, max_q must not be negative")
     _need(table.shape[1] * P < 2 ** 31, what, "the table holds more than 2^31 tokens")
-    if out is None:
+    fresh = out is None
+    if fresh:
         _chk_dev(q)
-        out = torch.zeros((rows, heads * hd), dtype=bf16, device=q.device)
+        out = torch.empty((rows, heads * hd), dtype=bf16, device=q.device)
     else:
         _need(out.dtype == bf16 and tuple(out.shape) == (rows, heads * hd) and (out.stride(1) == 1 or out.numel() == 0) and _own_elements(out), what,
               f"out must be bf16 [{rows}, {heads * hd}], its rows contiguous and apart")
@@ -1411,7 +1418,11 @@ def kv4_attn(q, cache, table, kv_len, cu_q, max_q, alpha, *, max_len=None, out=N
     p.q, p.codes, p.scales, p.table, p.kv_len, p.cu_q, p.out = (_p(t) for t in (q, cache.codes, cache.scales, table, kv_len, cu_q, out))
     p.sq_row, p.sq_head, p.so_row, p.ld_table = q.stride(0), q.stride(1), out.stride(0), max(table.stride(0), table.shape[1])
     p.requests, p.heads, p.kv, p.hd, p.page, p.pages, p.max_pages = B, heads, kv, hd, P, pages, table.shape[1]
-    p.rows, p.max_q, p.n_split, p.alpha = rows, max_q, 1, float(alpha)
+    n_split = _kv4_split(B * kv, table.shape[1] * P if max_len is None else max_len, max_q * (heads // kv))
+    if n_split > 1:
+        partial = torch.empty(rows * heads * n_split * (hd + 2), dtype=torch.float32, device=q.device)
+        p.partial = _p(partial)
+    p.rows, p.max_q, p.n_split, p.fresh, p.alpha = rows, max_q, n_split, int(fresh), float(alpha)
     _lib.check(_lib.lib().grove_kv4_attn(C.byref(p), _stream()), "grove_kv4_attn")
     return out
 

@@ -724,6 +724,7 @@ typedef struct grove_kv4_attn_params {
   float* partial;
   int64_t sq_row, sq_head, so_row, ld_table;
   int32_t requests, heads, kv, hd, page, pages, max_pages, rows, max_q, n_split;
+  int32_t fresh; /* 1: out is a new tensor, its rows of no request are set to 0 */
   float alpha;
 } grove_kv4_attn_params;
 int grove_kv4_attn(const grove_kv4_attn_params* p, void* stream);
