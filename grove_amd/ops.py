@@ -1181,22 +1181,41 @@ def sumsq(x, out=None):
 
 
 # ---- serving from a paged 4-bit cache with drafted tokens (grove_hip.h "Serving from a paged 4-bit key / value cache")
-def _need(cond, what, msg):
-    if not cond:
-        raise RuntimeError(f"{what}: {msg}")
+# A decode step calls these for every layer with little work in each, so what the host spends per call counts: messages are made only
+# where a call is refused, the params struct is filled in one go, the entry and the stream are looked up without a detour.
+def _refuse(what, msg):
+    raise RuntimeError(f"{what}: {msg}")
 
 
-def _one_device(what, *ts):
-    """Every tensor on the CURRENT device: a launch goes to it, whatever device its tensors are on."""
-    _chk_dev(*ts)
-    cur = torch.cuda.current_device()
+_entries = {}
+
+
+def _launch(name, params, *ts):
+    """Calls grove_<name>. Every tensor must be on the CURRENT device: the launch goes to its current stream, wherever the tensors are."""
+    if ts[0].get_device() < 0:
+        raise RuntimeError(f"{name}: grove_amd ops need device tensors (no CPU fallback exists)")
+    cur = torch._C._cuda_getDevice()
     for t in ts:
-        _need(t is None or t.device.index == cur, what, f"a tensor is on {t.device if t is not None else None}, the current device is cuda:{cur}")
+        if t is not None and t.get_device() != cur:
+            _refuse(name, f"a tensor is on {t.device}, the current device is cuda:{cur}")
+    fn = _entries.get(name)
+    if fn is None:
+        fn = getattr(_lib.lib(), "grove_" + name)
+        fn.argtypes = [C.c_void_p, C.c_void_p]
+        _entries[name] = fn
+    rc = fn(C.byref(params), torch._C._cuda_getCurrentRawStream(cur))
+    if rc:
+        _lib.check(rc, "grove_" + name)
 
 
-def _lens(what, n, **ts):
-    for name, t in ts.items():
-        _need(t.dtype == torch.int32 and t.dim() == 1 and t.shape[0] == n and t.is_contiguous(), what, f"{name} must be contiguous int32 [{n}]")
+def _need_device(what, t):
+    if t.get_device() < 0:
+        raise RuntimeError(f"{what}: grove_amd ops need device tensors (no CPU fallback exists)")
+
+
+def _lens(what, name, t, n):
+    if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous():
+        _refuse(what, f"{name} must be contiguous int32 [{n}]")
 
 
 def _span(t):
@@ -1212,6 +1231,8 @@ def _apart(a, b):
 
 def _own_elements(t):
     """No two elements of a view share memory (a broadcast view must not be written)."""
+    if t.is_contiguous():
+        return True
     at = 1
     for s, n in sorted((s, n) for s, n in zip(t.stride(), t.shape) if n > 1):
         if s < at:
@@ -1234,21 +1255,27 @@ def rotary_plan(rot, theta=10000.0, *, interleaved=False, scaling="none", factor
     divides the pairs that turn less than `slow` times in trained_len, leaves those that turn more than `fast` times, blends linearly over
     the pair number between, and scales the rotated channels by 0.1 ln(factor) + 1 (Peng et al. 2023)."""
     what = "rotary_plan"
-    _need(rot >= 2 and rot % 2 == 0, what, f"rot = {rot} must be even and positive")
-    _need(scaling in ("none", "linear", "ntk", "yarn"), what, f"unknown scaling {scaling!r}")
-    _need(theta > 1.0 and factor >= 1.0, what, "theta must pass 1 and factor must not be below 1")
-    _need(scaling != "none" or factor == 1.0, what, "a factor needs a scaling")
+    if rot < 2 or rot % 2:
+        _refuse(what, f"rot = {rot} must be even and positive")
+    if scaling not in ("none", "linear", "ntk", "yarn"):
+        _refuse(what, f"unknown scaling {scaling!r}")
+    if not (theta > 1.0 and factor >= 1.0):
+        _refuse(what, "theta must pass 1 and factor must not be below 1")
+    if scaling == "none" and factor != 1.0:
+        _refuse(what, "a factor needs a scaling")
     mscale = 1.0
     if scaling == "ntk":
-        _need(rot > 2, what, "ntk needs rot > 2")
+        if rot == 2:
+            _refuse(what, "ntk needs rot > 2")
         theta = theta * factor ** (rot / (rot - 2))
     w = theta ** -(torch.arange(0, rot, 2, dtype=torch.float64) / rot)
     if scaling == "linear":
         w = w / factor
     elif scaling == "yarn":
-        _need(trained_len > 0 and fast > slow > 0, what, "yarn needs trained_len > 0 and fast > slow > 0")
+        if not (trained_len > 0 and fast > slow > 0):
+            _refuse(what, "yarn needs trained_len > 0 and fast > slow > 0")
 
-        def pair(turns):  # the (real) pair number, times two, that turns so many times in trained_len
+        def pair(turns):  # the (real) number of the pair that turns so many times in trained_len
             return rot * math.log(trained_len / (turns * 2 * math.pi)) / (2 * math.log(theta))
         low, high = max(math.floor(pair(fast)), 0), min(math.ceil(pair(slow)), rot - 1)
         ramp = ((torch.arange(rot // 2, dtype=torch.float64) - low) / max(high - low, 0.001)).clamp(0, 1)
@@ -1262,27 +1289,32 @@ def rotary(x, pos, plan, *, backward=False, out=None):
     [rows] (grove_rotary). out None: a new tensor; out = x (the same view): in place; any other out must not overlap x. backward: the gradient
     w.r.t. x for x = the gradient w.r.t. the result."""
     what = "rotary"
-    _need(x.dim() == 3 and x.dtype in (bf16, torch.float32), what, "x must be bf16 or f32 [rows, heads, hd]")
+    dt = x.dtype
+    if x.dim() != 3 or (dt != bf16 and dt != torch.float32):
+        _refuse(what, "x must be bf16 or f32 [rows, heads, hd]")
     rows, heads, hd = x.shape
-    _need(x.stride(2) == 1 or hd == 1 or x.numel() == 0, what, "the channels must be contiguous")
-    f = plan.freq
-    _need(f.dtype == torch.float64 and f.dim() == 1 and f.is_contiguous() and 0 < 2 * f.shape[0] <= hd, what, f"the plan must hold 1 to {hd // 2} f64 frequencies")
-    _lens(what, rows, pos=pos)
+    sr, sh, sc = x.stride()
+    if sc != 1 and hd > 1 and x.numel():
+        _refuse(what, "the channels must be contiguous")
+    f, interleaved, mscale = plan
+    if f.dtype != torch.float64 or f.dim() != 1 or not f.is_contiguous() or not 0 < 2 * f.shape[0] <= hd:
+        _refuse(what, f"the plan must hold 1 to {hd // 2} f64 frequencies, contiguous")
+    _lens(what, "pos", pos, rows)
     if out is None:
-        _chk_dev(x)
-        out = torch.empty((rows, heads, hd), dtype=x.dtype, device=x.device)
+        _need_device(what, x)
+        out = torch.empty((rows, heads, hd), dtype=dt, device=x.device)
+        yr, yh = heads * hd, hd
     else:
-        _need(out.shape == x.shape and out.dtype == x.dtype and (out.stride(2) == 1 or out.numel() == 0), what, "out must match x, its channels contiguous")
-        _need(_own_elements(out), what, "out has elements that share memory")
-        same = out.data_ptr() == x.data_ptr() and out.stride() == x.stride()
-        _need(same or _apart(out, x), what, "out overlaps x and is not the same view")
-    _one_device(what, x, pos, f, out)
-    p = _lib.RotaryParams()
-    p.x, p.y, p.pos, p.freq = _p(x), _p(out), _p(pos), _p(f)
-    p.sx_row, p.sx_head, p.sy_row, p.sy_head = x.stride(0), x.stride(1), out.stride(0), out.stride(1)
-    p.rows, p.heads, p.hd, p.rot = rows, heads, hd, 2 * f.shape[0]
-    p.interleaved, p.backward, p.f32, p.mscale = int(plan.interleaved), int(backward), int(x.dtype == torch.float32), float(plan.mscale)
-    _lib.check(_lib.lib().grove_rotary(C.byref(p), _stream()), "grove_rotary")
+        if out.shape != x.shape or out.dtype != dt or (out.stride(2) != 1 and hd > 1 and out.numel()):
+            _refuse(what, "out must match x, its channels contiguous")
+        if not _own_elements(out):
+            _refuse(what, "out has elements that share memory")
+        yr, yh = out.stride(0), out.stride(1)
+        if not (out.data_ptr() == x.data_ptr() and yr == sr and yh == sh) and not _apart(out, x):
+            _refuse(what, "out overlaps x and is not the same view")
+    p = _lib.RotaryParams(x.data_ptr(), out.data_ptr(), pos.data_ptr(), f.data_ptr(), sr, sh, yr, yh, rows, heads, hd, 2 * f.shape[0],
+                          interleaved, backward, dt == torch.float32, mscale)
+    _launch(what, p, x, pos, f, out)
     return out
 
 
@@ -1302,25 +1334,33 @@ def page_tables(ctx_len, new_len, table, held, free, page_size, rows):
     page numbers, used from the front; rows: the rows of the step, sum(new_len), or more for a step of fixed size. The caller drops the first
     `taken` of `free` (taken > len(free): the pages ran out, the rows without a page have slot -1)."""
     what = "page_tables"
-    _need(table.dim() == 2 and table.dtype == torch.int32 and table.shape[0] > 0 and table.shape[1] > 0 and table.stride(1) == 1 and _own_elements(table),
-          what, "table must be int32 [requests, max_pages], its rows contiguous and apart")
-    B = table.shape[0]
-    _lens(what, B, ctx_len=ctx_len, new_len=new_len, held=held)
-    _need(free.dtype == torch.int32 and free.dim() == 1 and free.is_contiguous(), what, "free must be contiguous int32")
-    _need(B <= 4096, what, f"{B} requests: at most 4096")
-    _need(page_size >= 1 and page_size & (page_size - 1) == 0, what, "the page size must be a power of two")
-    _need(0 <= rows < 2 ** 31, what, "bad number of rows")
-    _need(all(_apart(table, t) for t in (ctx_len, new_len, held, free)), what, "table overlaps an input")
-    _one_device(what, ctx_len, new_len, table, held, free)
+    if table.dim() != 2 or table.dtype != torch.int32 or 0 in table.shape or table.stride(1) != 1 or not _own_elements(table):
+        _refuse(what, "table must be int32 [requests, max_pages], its rows contiguous and apart")
+    B, most = table.shape
+    _lens(what, "ctx_len", ctx_len, B)
+    _lens(what, "new_len", new_len, B)
+    _lens(what, "held", held, B)
+    _lens(what, "free", free, free.numel())
+    if B > 4096:
+        _refuse(what, f"{B} requests: at most 4096")
+    if page_size < 1 or page_size & (page_size - 1):
+        _refuse(what, "the page size must be a power of two")
+    if not 0 <= rows < 2 ** 31:
+        _refuse(what, "bad number of rows")
+    ld = max(table.stride(0), most)
+    t0 = table.data_ptr()
+    t1 = t0 + 4 * ((B - 1) * ld + most)
+    at = [t.data_ptr() for t in (ctx_len, new_len, held, free)]
+    for a, n in zip(at, (B, B, B, free.shape[0])):
+        if a < t1 and a + 4 * n > t0:
+            _refuse(what, "table overlaps an input")
+    _need_device(what, table)
     o = torch.empty(3 * B + 2 + 2 * rows, dtype=torch.int32, device=table.device)  # one allocation for the six results
-    step = PageStep(*o.split([B, B + 1, rows, rows, B, 1]))
-    p = _lib.PageTablesParams()
-    p.ctx_len, p.new_len, p.held, p.free_pages, p.table = _p(ctx_len), _p(new_len), _p(held), _p(free), _p(table)
-    p.kv_len, p.cu_q, p.slots, p.pos, p.held_out, p.taken = (_p(t) for t in step)
-    p.ld_table = max(table.stride(0), table.shape[1])
-    p.requests, p.max_pages, p.page, p.rows, p.n_free = B, table.shape[1], page_size, rows, free.shape[0]
-    _lib.check(_lib.lib().grove_page_tables(C.byref(p), _stream()), "grove_page_tables")
-    return step
+    o0 = o.data_ptr()
+    o1, o2, o3, o4, o5 = o0 + 4 * B, o0 + 8 * B + 4, o0 + 8 * B + 4 + 4 * rows, o0 + 8 * B + 4 + 8 * rows, o0 + 12 * B + 4 + 8 * rows
+    p = _lib.PageTablesParams(*at, t0, o0, o1, o2, o3, o4, o5, ld, B, most, page_size, rows, free.shape[0])
+    _launch(what, p, table, ctx_len, new_len, held, free)
+    return PageStep(*o.split_with_sizes((B, B + 1, rows, rows, B, 1)))
 
 
 class KV4Cache(NamedTuple):
@@ -1330,9 +1370,13 @@ class KV4Cache(NamedTuple):
     scales: torch.Tensor
 
 
+_PAGES, _HEADS = (16, 32, 64, 128, 256), (32, 64, 128, 256)
+
+
 def kv4_cache(pages, page_size, kv, hd, device):
     """An empty 4-bit cache of `pages` pages for `kv` key / value heads of hd channels."""
-    _need(page_size in (16, 32, 64, 128, 256) and hd in (32, 64, 128, 256), "kv4_cache", "the page must hold 16 to 256 tokens, the head 32, 64, 128 or 256 channels")
+    if page_size not in _PAGES or hd not in _HEADS:
+        _refuse("kv4_cache", "the page must hold 16, 32, 64, 128 or 256 tokens, the head 32, 64, 128 or 256 channels")
     return KV4Cache(torch.zeros((pages, 2, kv, page_size * hd // 2), dtype=torch.uint8, device=device),
                     torch.zeros((pages, 2, kv, page_size, 2), dtype=bf16, device=device))
 
@@ -1340,12 +1384,13 @@ def kv4_cache(pages, page_size, kv, hd, device):
 def _kv4_shape(what, cache):
     """(pages, kv, page_size, hd) of a cache."""
     c, s = cache
-    _need(c.dtype == torch.uint8 and c.dim() == 4 and c.is_contiguous() and s.dtype == bf16 and s.dim() == 5 and s.is_contiguous(), what,
-          "the cache must be a KV4Cache of contiguous tensors")
-    pages, two, kv, P = s.shape[:4]
-    _need(two == 2 and s.shape[4] == 2 and c.shape[:3] == s.shape[:3] and pages > 0 and kv > 0 and P in (16, 32, 64, 128, 256), what, "codes and scales do not fit each other")
-    hd = 2 * c.shape[3] // P
-    _need(hd in (32, 64, 128, 256) and hd * P == 2 * c.shape[3], what, "the head must have 32, 64, 128 or 256 channels")
+    if c.dtype != torch.uint8 or c.dim() != 4 or not c.is_contiguous() or s.dtype != bf16 or s.dim() != 5 or not s.is_contiguous():
+        _refuse(what, "the cache must be a KV4Cache of contiguous tensors")
+    pages, two, kv, P, pair = s.shape
+    n0, n1, n2, row = c.shape
+    hd = 2 * row // P if P in _PAGES else 0
+    if two != 2 or pair != 2 or n0 != pages or n1 != 2 or n2 != kv or pages == 0 or kv == 0 or hd not in _HEADS or hd * P != 2 * row:
+        _refuse(what, "codes and scales do not fit each other")
     return pages, kv, P, hd
 
 
@@ -1354,32 +1399,38 @@ def kv4_append(k, v, cache, slots):
     page_size + offset; one outside the cache is skipped, the others are distinct) (grove_kv4_append)."""
     what = "kv4_append"
     pages, kv, P, hd = _kv4_shape(what, cache)
+    rows = k.shape[0]
     for t in (k, v):
-        _need(t.dtype == bf16 and t.dim() == 3 and tuple(t.shape[1:]) == (kv, hd) and (t.stride(2) == 1 or t.numel() == 0), what,
-              f"k and v must be bf16 [rows, {kv}, {hd}], the channels contiguous")
-    _need(k.shape[0] == v.shape[0], what, "k and v differ in rows")
-    _lens(what, k.shape[0], slots=slots)
-    _need(all(_apart(t, c) for t in (k, v, slots) for c in cache), what, "an input lies in the cache")
-    _one_device(what, k, v, cache.codes, cache.scales, slots)
-    p = _lib.Kv4AppendParams()
-    p.k, p.v, p.codes, p.scales, p.slots = _p(k), _p(v), _p(cache.codes), _p(cache.scales), _p(slots)
-    p.sk_row, p.sk_head, p.sv_row, p.sv_head = k.stride(0), k.stride(1), v.stride(0), v.stride(1)
-    p.rows, p.kv, p.hd, p.page, p.pages = k.shape[0], kv, hd, P, pages
-    _lib.check(_lib.lib().grove_kv4_append(C.byref(p), _stream()), "grove_kv4_append")
+        if t.dtype != bf16 or t.dim() != 3 or t.shape[1] != kv or t.shape[2] != hd or (t.stride(2) != 1 and t.numel()):
+            _refuse(what, f"k and v must be bf16 [rows, {kv}, {hd}], the channels contiguous")
+    if v.shape[0] != rows:
+        _refuse(what, "k and v differ in rows")
+    _lens(what, "slots", slots, rows)
+    codes, scales = cache
+    kp, vp, sp, c0, s0 = k.data_ptr(), v.data_ptr(), slots.data_ptr(), codes.data_ptr(), scales.data_ptr()
+    c1, s1 = c0 + codes.numel(), s0 + 2 * scales.numel()
+    for a in (kp, vp, sp):
+        if c0 <= a < c1 or s0 <= a < s1:
+            _refuse(what, "an input lies in the cache")
+    kr, kh, _ = k.stride()
+    vr, vh, _ = v.stride()
+    _launch(what, _lib.Kv4AppendParams(kp, vp, c0, s0, sp, kr, kh, vr, vh, rows, kv, hd, P, pages), k, v, codes, scales, slots)
 
 
 def kv4_read(cache, slots, out_dtype=bf16):
     """(k, v) [rows, kv, hd], bf16 or f32: the values that the cache rows `slots` stand for; a slot outside the cache reads as zeros (grove_kv4_read)."""
     what = "kv4_read"
     pages, kv, P, hd = _kv4_shape(what, cache)
-    _need(out_dtype in (bf16, torch.float32), what, "out_dtype must be bf16 or f32")
-    _lens(what, slots.numel(), slots=slots)
-    _one_device(what, cache.codes, cache.scales, slots)
-    k, v = (torch.empty((slots.shape[0], kv, hd), dtype=out_dtype, device=slots.device) for _ in range(2))
-    p = _lib.Kv4ReadParams()
-    p.codes, p.scales, p.slots, p.k, p.v = _p(cache.codes), _p(cache.scales), _p(slots), _p(k), _p(v)
-    p.rows, p.kv, p.hd, p.page, p.pages, p.f32 = slots.shape[0], kv, hd, P, pages, int(out_dtype == torch.float32)
-    _lib.check(_lib.lib().grove_kv4_read(C.byref(p), _stream()), "grove_kv4_read")
+    if out_dtype != bf16 and out_dtype != torch.float32:
+        _refuse(what, "out_dtype must be bf16 or f32")
+    rows = slots.numel()
+    _lens(what, "slots", slots, rows)
+    _need_device(what, slots)
+    codes, scales = cache
+    k = torch.empty((rows, kv, hd), dtype=out_dtype, device=slots.device)
+    v = torch.empty((rows, kv, hd), dtype=out_dtype, device=slots.device)
+    p = _lib.Kv4ReadParams(codes.data_ptr(), scales.data_ptr(), slots.data_ptr(), k.data_ptr(), v.data_ptr(), rows, kv, hd, P, pages, out_dtype == torch.float32)
+    _launch(what, p, slots, codes, scales)
     return k, v
 
 
@@ -1396,34 +1447,40 @@ def kv4_attn(q, cache, table, kv_len, cu_q, max_q, alpha, *, max_len=None, out=N
     split of the work goes by it. Returns bf16 [rows, heads * hd]; rows of no request are zero in a new tensor and stay as they were in `out`."""
     what = "kv4_attn"
     pages, kv, P, hd = _kv4_shape(what, cache)
-    _need(q.dtype == bf16 and q.dim() == 3 and q.shape[2] == hd and q.shape[1] % kv == 0 and q.shape[1] > 0, what, f"q must be bf16 [rows, a multiple of {kv}, {hd}]")
-    _need(q.stride(2) == 1 or q.numel() == 0, what, "the channels must be contiguous")
-    _need(table.dim() == 2 and table.dtype == torch.int32 and table.shape[0] > 0 and table.shape[1] > 0 and table.stride(1) == 1, what,
-          "table must be int32 [requests, max_pages], its rows contiguous")
-    B, rows, heads = table.shape[0], q.shape[0], q.shape[1]
-    _lens(what, B, kv_len=kv_len)
-    _lens(what, B + 1, cu_q=cu_q)
-    _need(B <= 65535 and max_q >= 0, what, "at most 65535 requests, max_q must not be negative")
-    _need(table.shape[1] * P < 2 ** 31, what, "the table holds more than 2^31 tokens")
+    if q.dtype != bf16 or q.dim() != 3 or q.shape[2] != hd or q.shape[1] % kv or q.shape[1] == 0:
+        _refuse(what, f"q must be bf16 [rows, a multiple of {kv}, {hd}]")
+    rows, heads, _ = q.shape
+    qr, qh, qc = q.stride()
+    if qc != 1 and q.numel():
+        _refuse(what, "the channels must be contiguous")
+    if table.dim() != 2 or table.dtype != torch.int32 or 0 in table.shape or table.stride(1) != 1:
+        _refuse(what, "table must be int32 [requests, max_pages], its rows contiguous")
+    B, most = table.shape
+    _lens(what, "kv_len", kv_len, B)
+    _lens(what, "cu_q", cu_q, B + 1)
+    if B > 65535 or max_q < 0:
+        _refuse(what, "at most 65535 requests, max_q must not be negative")
+    if most * P >= 2 ** 31:
+        _refuse(what, "the table holds more than 2^31 tokens")
+    codes, scales = cache
     fresh = out is None
     if fresh:
-        _chk_dev(q)
+        _need_device(what, q)
         out = torch.empty((rows, heads * hd), dtype=bf16, device=q.device)
+        orow = heads * hd
     else:
-        _need(out.dtype == bf16 and tuple(out.shape) == (rows, heads * hd) and (out.stride(1) == 1 or out.numel() == 0) and _own_elements(out), what,
-              f"out must be bf16 [{rows}, {heads * hd}], its rows contiguous and apart")
-        _need(all(_apart(out, t) for t in (q, cache.codes, cache.scales, table, kv_len, cu_q)), what, "out overlaps an input")
-    _one_device(what, q, cache.codes, cache.scales, table, kv_len, cu_q, out)
-    p = _lib.Kv4AttnParams()
-    p.q, p.codes, p.scales, p.table, p.kv_len, p.cu_q, p.out = (_p(t) for t in (q, cache.codes, cache.scales, table, kv_len, cu_q, out))
-    p.sq_row, p.sq_head, p.so_row, p.ld_table = q.stride(0), q.stride(1), out.stride(0), max(table.stride(0), table.shape[1])
-    p.requests, p.heads, p.kv, p.hd, p.page, p.pages, p.max_pages = B, heads, kv, hd, P, pages, table.shape[1]
-    n_split = _kv4_split(B * kv, table.shape[1] * P if max_len is None else max_len, max_q * (heads // kv))
-    if n_split > 1:
-        partial = torch.empty(rows * heads * n_split * (hd + 2), dtype=torch.float32, device=q.device)
-        p.partial = _p(partial)
-    p.rows, p.max_q, p.n_split, p.fresh, p.alpha = rows, max_q, n_split, int(fresh), float(alpha)
-    _lib.check(_lib.lib().grove_kv4_attn(C.byref(p), _stream()), "grove_kv4_attn")
+        if out.dtype != bf16 or out.dim() != 2 or out.shape[0] != rows or out.shape[1] != heads * hd or (out.stride(1) != 1 and out.numel()) or not _own_elements(out):
+            _refuse(what, f"out must be bf16 [{rows}, {heads * hd}], its rows contiguous and apart")
+        if not all(_apart(out, t) for t in (q, codes, scales, table, kv_len, cu_q)):
+            _refuse(what, "out overlaps an input")
+        orow = out.stride(0)
+    n_split = _kv4_split(B * kv, most * P if max_len is None else max_len, max_q * (heads // kv))
+    # the joined splits' workspace: from the allocator at every call, so that calls on other streams and captured graphs have their own
+    partial = torch.empty(rows * heads * n_split * (hd + 2), dtype=torch.float32, device=q.device) if n_split > 1 else None
+    p = _lib.Kv4AttnParams(q.data_ptr(), codes.data_ptr(), scales.data_ptr(), table.data_ptr(), kv_len.data_ptr(), cu_q.data_ptr(), out.data_ptr(),
+                           0 if partial is None else partial.data_ptr(), qr, qh, orow, max(table.stride(0), most), B, heads, kv, hd, P, pages, most,
+                           rows, max_q, n_split, fresh, alpha)
+    _launch(what, p, q, codes, scales, table, kv_len, cu_q, out)
     return out
 
 
@@ -1433,26 +1490,28 @@ def verify_drafts(draft, q, p, u, pick, count=None):
     drafter that is certain of its token; p [requests, drafts + 1, vocab] the target's, of the same type; u f32 [requests, drafts] and pick f32
     [requests] uniform numbers of [0, 1); count int32 [requests]: drafts that a request has (default: all)."""
     what = "verify_drafts"
-    _need(draft.dtype == torch.int32 and draft.dim() == 2 and draft.is_contiguous(), what, "draft must be contiguous int32 [requests, drafts]")
+    if draft.dtype != torch.int32 or draft.dim() != 2 or not draft.is_contiguous():
+        _refuse(what, "draft must be contiguous int32 [requests, drafts]")
     B, K = draft.shape
-    _need(p.dtype in (bf16, torch.float32) and p.dim() == 3 and tuple(p.shape[:2]) == (B, K + 1) and p.shape[2] > 0 and p.stride(2) == 1, what,
-          f"p must be f32 or bf16 [{B}, {K + 1}, vocab], its rows contiguous")
+    dt = p.dtype
+    if (dt != bf16 and dt != torch.float32) or p.dim() != 3 or p.shape[0] != B or p.shape[1] != K + 1 or p.shape[2] == 0 or p.stride(2) != 1:
+        _refuse(what, f"p must be f32 or bf16 [{B}, {K + 1}, vocab], its rows contiguous")
     V = p.shape[2]
-    if K == 0:
-        q = None
-    _need(q is None or (q.dtype == p.dtype and tuple(q.shape) == (B, K, V) and q.stride(2) == 1), what, f"q must have p's type and be [{B}, {K}, {V}], its rows contiguous")
-    _need(u.dtype == torch.float32 and tuple(u.shape) == (B, K) and u.is_contiguous(), what, f"u must be contiguous f32 [{B}, {K}]")
-    _need(pick.dtype == torch.float32 and tuple(pick.shape) == (B,) and pick.is_contiguous(), what, f"pick must be contiguous f32 [{B}]")
+    qp = qb = qr = 0
+    if q is not None and K:
+        if q.dtype != dt or q.dim() != 3 or q.shape[0] != B or q.shape[1] != K or q.shape[2] != V or q.stride(2) != 1:
+            _refuse(what, f"q must have p's type and be [{B}, {K}, {V}], its rows contiguous")
+        qp, qb, qr = q.data_ptr(), q.stride(0), q.stride(1)
+    if u.dtype != torch.float32 or u.shape != draft.shape or not u.is_contiguous():
+        _refuse(what, f"u must be contiguous f32 [{B}, {K}]")
+    if pick.dtype != torch.float32 or pick.dim() != 1 or pick.shape[0] != B or not pick.is_contiguous():
+        _refuse(what, f"pick must be contiguous f32 [{B}]")
     if count is not None:
-        _lens(what, B, count=count)
-    _one_device(what, draft, q, p, u, pick, count)
+        _lens(what, "count", count, B)
+    _need_device(what, p)
     tokens = torch.empty((B, K + 1), dtype=torch.int32, device=p.device)
     accepted = torch.empty(B, dtype=torch.int32, device=p.device)
-    a = _lib.VerifyDraftsParams()
-    a.draft, a.q, a.p, a.u, a.pick, a.count, a.tokens, a.accepted = (_p(t) for t in (draft, q, p, u, pick, count, tokens, accepted))
-    a.sp_req, a.sp_row = p.stride(0), p.stride(1)
-    if q is not None:
-        a.sq_req, a.sq_row = q.stride(0), q.stride(1)
-    a.requests, a.drafts, a.vocab, a.bf16 = B, K, V, int(p.dtype == bf16)
-    _lib.check(_lib.lib().grove_verify_drafts(C.byref(a), _stream()), "grove_verify_drafts")
+    a = _lib.VerifyDraftsParams(draft.data_ptr(), qp, p.data_ptr(), u.data_ptr(), pick.data_ptr(), 0 if count is None else count.data_ptr(), tokens.data_ptr(),
+                                accepted.data_ptr(), qb, qr, p.stride(0), p.stride(1), B, K, V, dt == bf16)
+    _launch(what, a, p, draft, q if qp else None, u, pick, count)
     return tokens, accepted
