@@ -112,16 +112,24 @@ __device__ __forceinline__ void ld_words(unsigned* d, const unsigned char* a) {
     }
 }
 
-// Nibble j of either half of a word as a pair of bf16 16 + c: the nibble on mantissa bits 3..6 below the exponent of 16.
-__device__ __forceinline__ unsigned code_pair(unsigned w, int j) {
+// Nibble j of either half of a word as a pair of bf16 16 + c: the nibble on mantissa bits 3..6 below the exponent of 16. The two constants come
+// from registers that the compiler cannot look into: as literals they would not fit into one v_and_or_b32, and take two instructions.
+struct code_consts { unsigned mask, base; };
+__device__ __forceinline__ code_consts get_code_consts() {
+  code_consts k;
+  asm("s_mov_b32 %0, 0x780078" : "=s"(k.mask));
+  asm("v_mov_b32 %0, 0x41804180" : "=v"(k.base));
+  return k;
+}
+__device__ __forceinline__ unsigned code_pair(unsigned w, int j, const code_consts k) {
   const unsigned x = j == 0 ? w << 3 : w >> (4 * j - 3);
-  return (x & 0x00780078u) | 0x41804180u;
+  return (x & k.mask) | k.base;
 }
 __device__ __forceinline__ bf16x8_t frag(unsigned a, unsigned b, unsigned c, unsigned d) { return __builtin_bit_cast(bf16x8_t, (u32x4_t){a, b, c, d}); }
 
 constexpr float NEG = -INFINITY;
 
-constexpr int KV4_WAVES(int hd, int ct) { return hd * ct <= 128 ? 2 : 1; }
+constexpr int KV4_WAVES(int hd, int ct) { return hd * ct <= 64 ? 3 : hd * ct <= 128 ? 2 : 1; }
 
 template <int HD, int CT>
 __global__ __launch_bounds__(256, KV4_WAVES(HD, CT)) void kv4_attn_kernel(const grove_kv4_attn_params p, const int shift, const int vec_q, const int vec_o) {
@@ -146,7 +154,7 @@ __global__ __launch_bounds__(256, KV4_WAVES(HD, CT)) void kv4_attn_kernel(const 
   const int tiles = (seen_any + 31) >> 5, per = (tiles + p.n_split - 1) / p.n_split, tile0 = sp * per, tile1 = min(tiles, tile0 + per);
 
   bf16x8_t q[CT][NK];
-  float qs[CT], m[CT], l[CT], cst[CT];
+  float qs[CT], ref[CT], over[CT], l[CT], cst[CT];  // ref: taken off the scores; over: ref + 8, or -inf before the column's first key
   int lim[CT];
   const float a2 = p.alpha * 1.44269504088896340736f;
 #pragma unroll
@@ -170,8 +178,8 @@ __global__ __launch_bounds__(256, KV4_WAVES(HD, CT)) void kv4_attn_kernel(const 
     sum += __shfl_xor(sum, 32, 64);
     qs[ct] = sum * a2;
     lim[ct] = c < cols ? base + i : 0;
-    m[ct] = NEG;
-    l[ct] = cst[ct] = 0.f;
+    over[ct] = NEG;
+    ref[ct] = l[ct] = cst[ct] = 0.f;
   }
   f32x4_t acc[CT][NJ];
 #pragma unroll
@@ -179,142 +187,157 @@ __global__ __launch_bounds__(256, KV4_WAVES(HD, CT)) void kv4_attn_kernel(const 
 #pragma unroll
     for (int j = 0; j < NJ; ++j) acc[ct][j] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
 
-  // page numbers: 64 of them in the lanes, refilled when the wave has passed them
-  const int* row = p.table + b * p.ld_table;
-  int pg_lo = 0, pg_lane = -1;
-  bool have = false;
-  auto page_of = [&](int pi) -> int {  // pi: the same in all lanes, never below an earlier one
-    if (!have || pi >= pg_lo + 64) {
-      pg_lo = pi;
-      pg_lane = pi + lane < p.max_pages ? row[pi + lane] : -1;
-      have = true;
-    }
-    const int pg = __builtin_amdgcn_readlane(pg_lane, pi - pg_lo);
-    return pg >= 0 && pg < p.pages ? pg : -1;
-  };
+  // page numbers by scalar loads (the constant address space): asked for at a tile's start, used behind its scores for the next tile's keys. As
+  // vector loads they would be waited for together with the codes in flight.
+  typedef const __attribute__((address_space(4))) int* scalar_ints;
+  const scalar_ints row = (scalar_ints)(uintptr_t)(p.table + b * p.ld_table);
   const int P = 1 << shift;
-  auto load = [&](int tile, kv4_tile<HD>& T) {
+  const int64_t page_rows = (int64_t)2 * p.kv << shift, v_rows = (int64_t)p.kv << shift;  // cache rows of a page, and from its keys to its values
+  const unsigned char* codes = (const unsigned char*)p.codes + ((int64_t)hk << shift) * (HD / 2);
+  const unsigned* scales = (const unsigned*)p.scales + ((int64_t)hk << shift);
+  const code_consts kc = get_code_consts();
+  const int k_off = n16 * (HD / 2) + h * (HD / 8), v_off = h * (2 * HD) + n16 * (HD / 8);
+  int64_t at[2];   // cache rows of the tile whose keys were asked for last
+  int pg[2], ask[2];
+  kv4_tile<HD> T;
+  auto ask_pages = [&](int tile) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) ask[u] = row[min((tile * 32 + 16 * u) >> shift, p.max_pages - 1)];
+  };
+  // keys of a tile, then its values: the keys of the next tile are asked for when this one's scores are done, its values when these are summed
+  auto load_keys = [&](int tile) {
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      const int t = tile * 32 + 16 * u, pg = page_of(t >> shift), r = t & (P - 1);
-      T.page[u] = pg;
-      const int64_t plane = ((int64_t)max(pg, 0) * 2) * p.kv + hk;  // a missing page's keys are masked; its loads go to page 0
-      const unsigned char* kc = (const unsigned char*)p.codes + (plane << shift) * (HD / 2) + r * (HD / 2);
-      const unsigned char* vc = kc + ((int64_t)p.kv << shift) * (HD / 2);
-      ld_words<NK>(T.k[u], kc + n16 * (HD / 2) + h * (HD / 8));
-      ld_words<NK>(T.v[u], vc + h * (2 * HD) + n16 * (HD / 8));
-      const unsigned* sc = (const unsigned*)p.scales + (plane << shift) + r + 4 * h;
-      T.ks[u] = *(const u32x4_t*)sc;
-      T.vs[u] = *(const u32x4_t*)(sc + ((int64_t)p.kv << shift));
+      pg[u] = ask[u] >= 0 && ask[u] < p.pages ? ask[u] : -1;  // a missing page's keys are masked, its loads go to page 0
+      at[u] = max(pg[u], 0) * page_rows + ((tile * 32 + 16 * u) & (P - 1));
+      ld_words<NK>(T.k[u], codes + at[u] * (HD / 2) + k_off);
+      T.ks[u] = *(const u32x4_t*)(scales + at[u] + 4 * h);
     }
   };
-  auto compute = [&](int tile, const kv4_tile<HD>& T, auto masked) {
-    constexpr bool MASK = decltype(masked)::value;
-    float z[CT][8];
-    auto sees = [&](int ct, int u, int i) { return tile * 32 + 16 * u + 4 * h + i < lim[ct] && T.page[u] >= 0; };
+  auto load_values = [&]() {
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      __builtin_amdgcn_sched_barrier(0);  // one part's operands at a time: unpacked all at once they would take the registers of a third wave
-      bf16x8_t kf[NK];
-#pragma unroll
-      for (int t = 0; t < NK; ++t) kf[t] = frag(code_pair(T.k[u][t], 0), code_pair(T.k[u][t], 1), code_pair(T.k[u][t], 2), code_pair(T.k[u][t], 3));
-#pragma unroll
-      for (int ct = 0; ct < CT; ++ct) {
-        f32x4_t raw = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int t = 0; t < NK; ++t) raw = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[t], q[ct][t], raw, 0, 0, 0);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float s = bf_lo(T.ks[u][i]), mn = bf_hi(T.ks[u][i]);
-          float v = fmaf(raw[i], a2 * s, fmaf(-16.f, s, mn) * qs[ct]);
-          if constexpr (MASK) v = sees(ct, u, i) ? v : NEG;
-          z[ct][4 * u + i] = v;
-        }
-      }
+      T.page[u] = pg[u];
+      ld_words<NK>(T.v[u], codes + (at[u] + v_rows) * (HD / 2) + v_off);
+      T.vs[u] = *(const u32x4_t*)(scales + at[u] + v_rows + 4 * h);
     }
-    __builtin_amdgcn_sched_barrier(0);
-    float top[CT];
-    bool grow = false;
-#pragma unroll
-    for (int ct = 0; ct < CT; ++ct) {
-      top[ct] = z[ct][0];
-#pragma unroll
-      for (int i = 1; i < 8; ++i) top[ct] = fmaxf(top[ct], z[ct][i]);
-      grow |= top[ct] > m[ct] + 8.f;
-    }
-    if (__any(grow)) {
-#pragma unroll
-      for (int ct = 0; ct < CT; ++ct) {
-        float t = fmaxf(top[ct], __shfl_xor(top[ct], 16, 64));
-        t = fmaxf(t, __shfl_xor(t, 32, 64));
-        t = fmaxf(t, m[ct]);
-        const float f = m[ct] == NEG ? 0.f : __builtin_amdgcn_exp2f(m[ct] - t);
-        m[ct] = t;
-        l[ct] *= f;
-        cst[ct] *= f;
-#pragma unroll
-        for (int j = 0; j < NJ; ++j) acc[ct][j] *= f;
-      }
-    }
-    bf16x8_t hi[CT], lo[CT];
-#pragma unroll
-    for (int ct = 0; ct < CT; ++ct) {
-      const float ref = m[ct] == NEG ? 0.f : m[ct];
-      unsigned a[4], c[4];
+  };
+  // The tiles are run in two loops, with masks and without, and both are left where a score passes its column's maximum by 8: the accumulators are
+  // then rescaled between the loops and the tile is taken again. Branches around the rescaling or the masks inside one loop cost a copy of every
+  // accumulator per tile, and their merged paths a wait for the loads in flight.
+  int tile = tile0 + w;
+  float z[CT][8], top[CT];
+  auto needs_mask = [&]() { return ((tile + 1) * 32 > seen_all) | (T.page[0] < 0) | (T.page[1] < 0); };
+  auto run = [&](auto masked) -> bool {  // false: left for a rescaling
+    constexpr bool MASK = decltype(masked)::value;
+    while ((tile < tile1) & (needs_mask() == MASK)) {
+      const int next = min(tile + 4, tile1 - 1);  // (behind the last tile: an unused, valid one, so that the loads need no branch)
+      ask_pages(next);
+      auto sees = [&](int ct, int u, int i) { return (tile * 32 + 16 * u + 4 * h + i < lim[ct]) & (T.page[u] >= 0); };
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        float ps[4];
+        __builtin_amdgcn_sched_barrier(0);  // one part's operands at a time: unpacked all at once they would take the registers of a third wave
+        bf16x8_t kf[NK];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float e = __builtin_amdgcn_exp2f(z[ct][4 * u + i] - ref);
-          const float s = bf_lo(T.vs[u][i]), mn = fmaf(-16.f, s, bf_hi(T.vs[u][i]));
-          l[ct] += e;
-          ps[i] = e * s;
-          float pm = e * mn;
-          if constexpr (MASK) {  // an unseen row's scale may be anything
-            ps[i] = sees(ct, u, i) ? ps[i] : 0.f;
-            pm = sees(ct, u, i) ? pm : 0.f;
+        for (int t = 0; t < NK; ++t) kf[t] = frag(code_pair(T.k[u][t], 0, kc), code_pair(T.k[u][t], 1, kc), code_pair(T.k[u][t], 2, kc), code_pair(T.k[u][t], 3, kc));
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) {
+          f32x4_t raw = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int t = 0; t < NK; ++t) raw = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[t], q[ct][t], raw, 0, 0, 0);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float s = bf_lo(T.ks[u][i]), mn = bf_hi(T.ks[u][i]);
+            float v = fmaf(raw[i], a2 * s, fmaf(-16.f, s, mn) * qs[ct]);
+            if constexpr (MASK) v = sees(ct, u, i) ? v : NEG;
+            z[ct][4 * u + i] = v;
           }
-          cst[ct] += pm;
-        }
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          a[2 * u + i] = pack2bf(ps[2 * i], ps[2 * i + 1]);
-          c[2 * u + i] = pack2bf(ps[2 * i] - bf_lo(a[2 * u + i]), ps[2 * i + 1] - bf_hi(a[2 * u + i]));
         }
       }
-      hi[ct] = frag(a[0], a[1], a[2], a[3]);
-      lo[ct] = frag(c[0], c[1], c[2], c[3]);
-    }
-#pragma unroll
-    for (int j = 0; j < NJ; ++j) {
-      if ((j & 1) == 0) __builtin_amdgcn_sched_barrier(0);
-      bf16x8_t vf;
-      if constexpr (HD == 32) vf = frag(code_pair(T.v[0][0], j), code_pair(T.v[0][0], j + 2), code_pair(T.v[1][0], j), code_pair(T.v[1][0], j + 2));
-      else {
-        const int o = (j >> 2) * 2, jn = j & 3;
-        vf = frag(code_pair(T.v[0][o], jn), code_pair(T.v[0][o + 1], jn), code_pair(T.v[1][o], jn), code_pair(T.v[1][o + 1], jn));
-      }
+      bool grow = false;
 #pragma unroll
       for (int ct = 0; ct < CT; ++ct) {
-        acc[ct][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, hi[ct], acc[ct][j], 0, 0, 0);
-        acc[ct][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, lo[ct], acc[ct][j], 0, 0, 0);
+        top[ct] = z[ct][0];
+#pragma unroll
+        for (int i = 1; i < 8; ++i) top[ct] = fmaxf(top[ct], z[ct][i]);
+        grow |= top[ct] > over[ct];
       }
+      asm volatile("" ::"s"(ask[0]), "s"(ask[1]));  // (keeps the page numbers' loads at the top)
+      if (__any(grow)) return false;
+      __builtin_amdgcn_sched_barrier(0);
+      load_keys(next);
+      __builtin_amdgcn_sched_barrier(0);
+      bf16x8_t hi[CT], lo[CT];
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) {
+        unsigned a[4], c[4];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          float ps[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float e = __builtin_amdgcn_exp2f(z[ct][4 * u + i] - ref[ct]);
+            const float s = bf_lo(T.vs[u][i]), mn = fmaf(-16.f, s, bf_hi(T.vs[u][i]));
+            l[ct] += e;
+            ps[i] = e * s;
+            if constexpr (MASK) {  // an unseen row's scale may be anything
+              ps[i] = sees(ct, u, i) ? ps[i] : 0.f;
+              cst[ct] += sees(ct, u, i) ? e * mn : 0.f;
+            } else cst[ct] = fmaf(e, mn, cst[ct]);
+          }
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            a[2 * u + i] = pack2bf(ps[2 * i], ps[2 * i + 1]);
+            c[2 * u + i] = pack2bf(ps[2 * i] - bf_lo(a[2 * u + i]), ps[2 * i + 1] - bf_hi(a[2 * u + i]));
+          }
+        }
+        hi[ct] = frag(a[0], a[1], a[2], a[3]);
+        lo[ct] = frag(c[0], c[1], c[2], c[3]);
+      }
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) {
+        if ((j & 1) == 0) __builtin_amdgcn_sched_barrier(0);
+        bf16x8_t vf;
+        if constexpr (HD == 32) vf = frag(code_pair(T.v[0][0], j, kc), code_pair(T.v[0][0], j + 2, kc), code_pair(T.v[1][0], j, kc), code_pair(T.v[1][0], j + 2, kc));
+        else {
+          const int o = (j >> 2) * 2, jn = j & 3;
+          vf = frag(code_pair(T.v[0][o], jn, kc), code_pair(T.v[0][o + 1], jn, kc), code_pair(T.v[1][o], jn, kc), code_pair(T.v[1][o + 1], jn, kc));
+        }
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) {
+          acc[ct][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, hi[ct], acc[ct][j], 0, 0, 0);
+          acc[ct][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, lo[ct], acc[ct][j], 0, 0, 0);
+        }
+      }
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) asm volatile("" : "+v"(l[ct]), "+v"(cst[ct]));  // (their sums are not put off past the next loads)
+      __builtin_amdgcn_sched_barrier(0);
+      load_values();
+      tile += 4;
     }
+    return true;
   };
-
-  int tile = tile0 + w;
   if (tile < tile1) {
-    kv4_tile<HD> cur, nxt;
-    load(tile, cur);
-    while (true) {
-      const int next = tile + 4;
-      if (next < tile1) load(next, nxt);
-      if ((tile + 1) * 32 <= seen_all && cur.page[0] >= 0 && cur.page[1] >= 0) compute(tile, cur, std::false_type{});
-      else compute(tile, cur, std::true_type{});
-      if (next >= tile1) break;
-      cur = nxt;
-      tile = next;
+    ask_pages(tile);
+    load_keys(tile);
+    load_values();
+  }
+  while (tile < tile1) {
+    if (needs_mask() ? run(std::true_type{}) : run(std::false_type{})) continue;
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+      float t = fmaxf(top[ct], __shfl_xor(top[ct], 16, 64));
+      t = fmaxf(t, __shfl_xor(t, 32, 64));
+      const bool up = t > over[ct];
+      const float f = up && over[ct] != NEG ? __builtin_amdgcn_exp2f(ref[ct] - t) : 1.f;  // (before the first key there is nothing to rescale)
+      if (up) {
+        ref[ct] = t;
+        over[ct] = t + 8.f;
+      }
+      l[ct] *= f;
+      cst[ct] *= f;
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) acc[ct][j] *= f;
     }
   }
 
@@ -326,7 +349,7 @@ __global__ __launch_bounds__(256, KV4_WAVES(HD, CT)) void kv4_attn_kernel(const 
     cst[ct] += __shfl_xor(cst[ct], 16, 64);
     cst[ct] += __shfl_xor(cst[ct], 32, 64);
     if (h == 0) {
-      s_m[w][ct * 16 + n16] = m[ct];
+      s_m[w][ct * 16 + n16] = over[ct] == NEG ? NEG : ref[ct];
       s_l[w][ct * 16 + n16] = l[ct];
       s_c[w][ct * 16 + n16] = cst[ct];
     }
@@ -338,7 +361,7 @@ __global__ __launch_bounds__(256, KV4_WAVES(HD, CT)) void kv4_attn_kernel(const 
   for (int ct = 0; ct < CT; ++ct) {
     auto joint = [&](int col) { return fmaxf(fmaxf(s_m[0][col], s_m[1][col]), fmaxf(s_m[2][col], s_m[3][col])); };
     auto part = [&](float mw, float M) { return mw == NEG ? 0.f : __builtin_amdgcn_exp2f(mw - M); };
-    const float f = part(m[ct], joint(ct * 16 + n16));
+    const float f = part(s_m[w][ct * 16 + n16], joint(ct * 16 + n16));
     const int col = ct * 16 + oc, c = col0 + col, i = c / G;
     const float M = joint(col);
     float L = 0.f, C = 0.f;
