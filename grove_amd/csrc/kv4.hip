@@ -93,23 +93,59 @@ __global__ __launch_bounds__(64) void kv4_read_kernel(const grove_kv4_read_param
 //     4 h + i of either part in lane (col, h), and the values' four-token order gives the A operand the same keys. P s goes in as two bf16 parts
 //     (hi + lo, 2^-17), the minimum's share sum P (m - 16 s) is one number per column.
 // Running maximum in log2 units, raised only where a score passes it by 8 (P <= 2^8 keeps its precision in fp32): most tiles skip the rescaling.
+// The tiles travel global -> LDS (LDS-DMA) into a ring of kv4_slots slots per wave: several tiles per wave are in flight without a register held
+// for them, and every lane takes back the bytes that it asked for (its K and V pieces side by side in lane order: no bank conflicts, and no
+// barrier, since a wave reads only its own ring). Waits are counted: a tile is kv4_ops vector memory operations.
+constexpr int kv4_part(int hd) { return 64 * (hd / 8); }              // bytes of 16 keys' codes
+constexpr int kv4_bytes(int hd) { return 4 * kv4_part(hd) + 256; }    // of a tile: two parts of keys, two of values, scales
+constexpr int kv4_ops(int hd) { return 4 * (hd == 64 || hd == 256 ? 2 : 1) + 1; }
+constexpr int kv4_slots(int hd, int ct) { return hd == 256 ? (ct == 1 ? 2 : 4) : hd == 128 ? (ct == 1 ? 3 : ct == 2 ? 4 : 6) : 4; }
+
 template <int HD>
 struct kv4_tile {
   unsigned k[2][HD / 32], v[2][HD / 32];
   u32x4_t ks[2], vs[2];
-  int page[2];  // -1: not a page of the cache
 };
 
-template <int N>
-__device__ __forceinline__ void ld_words(unsigned* d, const unsigned char* a) {
-  if constexpr (N == 1) d[0] = *(const unsigned*)a;
-  else if constexpr (N == 2) { const u32x2_t x = *(const u32x2_t*)a; d[0] = x[0]; d[1] = x[1]; }
-  else
-#pragma unroll
-    for (int i = 0; i < N; i += 4) {
-      const u32x4_t x = *(const u32x4_t*)(a + 4 * i);
-      d[i] = x[0]; d[i + 1] = x[1]; d[i + 2] = x[2]; d[i + 3] = x[3];
+__device__ __forceinline__ void dma16(const void* g, char* lds) {
+  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)g, (__attribute__((address_space(3))) void*)lds, 16, 0, 0);
+}
+__device__ __forceinline__ void dma4(const void* g, char* lds) {
+  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)g, (__attribute__((address_space(3))) void*)lds, 4, 0, 0);
+}
+// Two parts' codes and their scales from the ring, waited for in place (the compiler would wait for every load in flight). O: offset of the codes
+// within the tile, OS: of the scales.
+template <int HD, int O, int OS>
+__device__ __forceinline__ void ring_read(unsigned a, unsigned as, unsigned (&w)[2][HD / 32], u32x4_t (&s)[2]) {
+  if constexpr (HD == 32) {
+    asm volatile("ds_read_b32 %0, %4 offset:%6\n\tds_read_b32 %1, %4 offset:%7\n\tds_read_b128 %2, %5 offset:%8\n\tds_read_b128 %3, %5 offset:%9\n\t"
+                 "s_waitcnt lgkmcnt(0)"
+                 : "=&v"(w[0][0]), "=&v"(w[1][0]), "=&v"(s[0]), "=&v"(s[1])
+                 : "v"(a), "v"(as), "n"(O), "n"(O + 256), "n"(OS), "n"(OS + 64) : "memory");
+  } else if constexpr (HD == 64) {
+    asm volatile("ds_read_b32 %0, %6 offset:%8\n\tds_read_b32 %1, %6 offset:%9\n\tds_read_b32 %2, %6 offset:%10\n\tds_read_b32 %3, %6 offset:%11\n\t"
+                 "ds_read_b128 %4, %7 offset:%12\n\tds_read_b128 %5, %7 offset:%13\n\ts_waitcnt lgkmcnt(0)"
+                 : "=&v"(w[0][0]), "=&v"(w[0][1]), "=&v"(w[1][0]), "=&v"(w[1][1]), "=&v"(s[0]), "=&v"(s[1])
+                 : "v"(a), "v"(as), "n"(O), "n"(O + 256), "n"(O + 512), "n"(O + 768), "n"(OS), "n"(OS + 64) : "memory");
+  } else {
+    constexpr int N = HD / 128;
+    u32x4_t x[2][N];
+    if constexpr (N == 1) {
+      asm volatile("ds_read_b128 %0, %4 offset:%6\n\tds_read_b128 %1, %4 offset:%7\n\tds_read_b128 %2, %5 offset:%8\n\tds_read_b128 %3, %5 offset:%9\n\t"
+                   "s_waitcnt lgkmcnt(0)"
+                   : "=&v"(x[0][0]), "=&v"(x[1][0]), "=&v"(s[0]), "=&v"(s[1])
+                   : "v"(a), "v"(as), "n"(O), "n"(O + 1024), "n"(OS), "n"(OS + 64) : "memory");
+    } else {
+      asm volatile("ds_read_b128 %0, %6 offset:%8\n\tds_read_b128 %1, %6 offset:%9\n\tds_read_b128 %2, %6 offset:%10\n\tds_read_b128 %3, %6 offset:%11\n\t"
+                   "ds_read_b128 %4, %7 offset:%12\n\tds_read_b128 %5, %7 offset:%13\n\ts_waitcnt lgkmcnt(0)"
+                   : "=&v"(x[0][0]), "=&v"(x[0][N - 1]), "=&v"(x[1][0]), "=&v"(x[1][N - 1]), "=&v"(s[0]), "=&v"(s[1])
+                   : "v"(a), "v"(as), "n"(O), "n"(O + 1024), "n"(O + 2048), "n"(O + 3072), "n"(OS), "n"(OS + 64) : "memory");
     }
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int i = 0; i < HD / 32; ++i) w[u][i] = x[u][i / 4][i % 4];
+  }
 }
 
 // Nibble j of either half of a word as a pair of bf16 16 + c: the nibble on mantissa bits 3..6 below the exponent of 16. The two constants come
@@ -129,13 +165,16 @@ __device__ __forceinline__ bf16x8_t frag(unsigned a, unsigned b, unsigned c, uns
 
 constexpr float NEG = -INFINITY;
 
-constexpr int KV4_WAVES(int hd, int ct) { return hd * ct <= 64 ? 3 : hd * ct <= 128 ? 2 : 1; }
+constexpr int KV4_WAVES(int hd, int ct) { return hd * ct <= 128 ? 3 : hd * ct <= 256 ? 2 : 1; }
 
 template <int HD, int CT>
 __global__ __launch_bounds__(256, KV4_WAVES(HD, CT)) void kv4_attn_kernel(const grove_kv4_attn_params p, const int shift, const int vec_q, const int vec_o) {
   constexpr int NK = HD / 32, NJ = HD / 16, HC = HD < 128 ? HD : 128;  // HC channels go through LDS at a time
+  constexpr int S = kv4_slots(HD, CT), BYTES = kv4_bytes(HD), OPS = kv4_ops(HD), PART = kv4_part(HD);
+  static_assert(4 * S * BYTES >= (int)sizeof(float) * 4 * 16 * (HC + 4), "the outputs pass through the rings' memory");
+  extern __shared__ __attribute__((aligned(1024))) char smem[];
   __shared__ float s_m[4][16 * CT], s_l[4][16 * CT], s_c[4][16 * CT];
-  __shared__ float s_o[4][16][HC + 4];
+  float(*s_o)[16][HC + 4] = (float(*)[16][HC + 4])smem;
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), n16 = lane & 15, h = lane >> 4;
   const int G = p.heads / p.kv, chunks = gridDim.y / p.kv, hk = blockIdx.y / chunks, cc = blockIdx.y - hk * chunks, b = blockIdx.z, sp = blockIdx.x;
   if (p.fresh && p.n_split == 1 && b == 0 && cc == 0) {  // a new result's rows of no request
@@ -187,8 +226,7 @@ __global__ __launch_bounds__(256, KV4_WAVES(HD, CT)) void kv4_attn_kernel(const 
 #pragma unroll
     for (int j = 0; j < NJ; ++j) acc[ct][j] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
 
-  // page numbers by scalar loads (the constant address space): asked for at a tile's start, used behind its scores for the next tile's keys. As
-  // vector loads they would be waited for together with the codes in flight.
+  // page numbers by scalar loads (the constant address space), asked for one tile ahead of their use
   typedef const __attribute__((address_space(4))) int* scalar_ints;
   const scalar_ints row = (scalar_ints)(uintptr_t)(p.table + b * p.ld_table);
   const int P = 1 << shift;
@@ -197,43 +235,56 @@ __global__ __launch_bounds__(256, KV4_WAVES(HD, CT)) void kv4_attn_kernel(const 
   const unsigned* scales = (const unsigned*)p.scales + ((int64_t)hk << shift);
   const code_consts kc = get_code_consts();
   const int k_off = n16 * (HD / 2) + h * (HD / 8), v_off = h * (2 * HD) + n16 * (HD / 8);
-  int64_t at[2];   // cache rows of the tile whose keys were asked for last
-  int pg[2], ask[2];
+  char* ring = smem + w * S * BYTES;
+  const unsigned ring_at = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)ring;
+  int ask[2], ahead = tile0 + w, to = 0;  // the tile to be asked for next, and its slot
+  unsigned bad = 0;                       // two bits a slot: a part whose page is not one of the cache (its keys are masked, its loads go to page 0)
+  auto ask_pages = [&]() {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) ask[u] = row[min((ahead * 32 + 16 * u) >> shift, p.max_pages - 1)];
+  };
+  auto issue = [&]() {
+    char* slot = ring + to * BYTES;
+    int64_t at[2];
+    unsigned miss = 0;
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const bool ok = (ask[u] >= 0) & (ask[u] < p.pages);
+      miss |= ok ? 0u : 1u << u;
+      at[u] = (int64_t)(ok ? ask[u] : 0) * page_rows + ((ahead * 32 + 16 * u) & (P - 1));
+      const unsigned char* kp = codes + at[u] * (HD / 2) + k_off;
+      const unsigned char* vp = codes + (at[u] + v_rows) * (HD / 2) + v_off;
+      char* kl = slot + u * PART;
+      if constexpr (HD >= 128) {
+#pragma unroll
+        for (int i = 0; i < HD / 128; ++i) { dma16(kp + 16 * i, kl + 1024 * i); dma16(vp + 16 * i, kl + 2 * PART + 1024 * i); }
+      } else {
+#pragma unroll
+        for (int i = 0; i < HD / 32; ++i) { dma4(kp + 4 * i, kl + 256 * i); dma4(vp + 4 * i, kl + 2 * PART + 256 * i); }
+      }
+    }
+    dma4(scales + ((h & 1) ? at[1] : at[0]) + (h >= 2 ? v_rows : 0) + n16, slot + 4 * PART);  // keys' parts 0, 1, values' parts 0, 1
+    bad = (bad & ~(3u << (2 * to))) | miss << (2 * to);
+    to = to == S - 1 ? 0 : to + 1;
+    ahead += 4;
+    ask_pages();
+  };
   kv4_tile<HD> T;
-  auto ask_pages = [&](int tile) {
-#pragma unroll
-    for (int u = 0; u < 2; ++u) ask[u] = row[min((tile * 32 + 16 * u) >> shift, p.max_pages - 1)];
-  };
-  // keys of a tile, then its values: the keys of the next tile are asked for when this one's scores are done, its values when these are summed
-  auto load_keys = [&](int tile) {
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      pg[u] = ask[u] >= 0 && ask[u] < p.pages ? ask[u] : -1;  // a missing page's keys are masked, its loads go to page 0
-      at[u] = max(pg[u], 0) * page_rows + ((tile * 32 + 16 * u) & (P - 1));
-      ld_words<NK>(T.k[u], codes + at[u] * (HD / 2) + k_off);
-      T.ks[u] = *(const u32x4_t*)(scales + at[u] + 4 * h);
-    }
-  };
-  auto load_values = [&]() {
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      T.page[u] = pg[u];
-      ld_words<NK>(T.v[u], codes + (at[u] + v_rows) * (HD / 2) + v_off);
-      T.vs[u] = *(const u32x4_t*)(scales + at[u] + v_rows + 4 * h);
-    }
-  };
+
   // The tiles are run in two loops, with masks and without, and both are left where a score passes its column's maximum by 8: the accumulators are
   // then rescaled between the loops and the tile is taken again. Branches around the rescaling or the masks inside one loop cost a copy of every
   // accumulator per tile, and their merged paths a wait for the loads in flight.
-  int tile = tile0 + w;
+  int tile = tile0 + w, from = 0;
   float z[CT][8], top[CT];
-  auto needs_mask = [&]() { return ((tile + 1) * 32 > seen_all) | (T.page[0] < 0) | (T.page[1] < 0); };
+  auto needs_mask = [&]() { return ((tile + 1) * 32 > seen_all) | ((bad >> (2 * from) & 3) != 0); };
   auto run = [&](auto masked) -> bool {  // false: left for a rescaling
     constexpr bool MASK = decltype(masked)::value;
     while ((tile < tile1) & (needs_mask() == MASK)) {
-      const int next = min(tile + 4, tile1 - 1);  // (behind the last tile: an unused, valid one, so that the loads need no branch)
-      ask_pages(next);
-      auto sees = [&](int ct, int u, int i) { return (tile * 32 + 16 * u + 4 * h + i < lim[ct]) & (T.page[u] >= 0); };
+      auto sees = [&](int ct, int u, int i) { return (tile * 32 + 16 * u + 4 * h + i < lim[ct]) & ((bad >> (2 * from + u) & 1) == 0); };
+      if (ahead - tile == 4 * (S - 1)) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(OPS * (S - 2)) : "memory");  // the tiles behind this one may be on their way
+      else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");                                                  // the last ones
+      const unsigned slot = ring_at + from * BYTES, at_codes = slot + lane * (HD < 128 ? 4 : 16), at_scales = slot + 16 * h;
+      ring_read<HD, 0, 4 * PART>(at_codes, at_scales, T.k, T.ks);
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         __builtin_amdgcn_sched_barrier(0);  // one part's operands at a time: unpacked all at once they would take the registers of a third wave
@@ -262,11 +313,9 @@ __global__ __launch_bounds__(256, KV4_WAVES(HD, CT)) void kv4_attn_kernel(const 
         for (int i = 1; i < 8; ++i) top[ct] = fmaxf(top[ct], z[ct][i]);
         grow |= top[ct] > over[ct];
       }
-      asm volatile("" ::"s"(ask[0]), "s"(ask[1]));  // (keeps the page numbers' loads at the top)
       if (__any(grow)) return false;
-      __builtin_amdgcn_sched_barrier(0);
-      load_keys(next);
-      __builtin_amdgcn_sched_barrier(0);
+      if (ahead < tile1) issue();
+      ring_read<HD, 2 * PART, 4 * PART + 128>(at_codes, at_scales, T.v, T.vs);
       bf16x8_t hi[CT], lo[CT];
 #pragma unroll
       for (int ct = 0; ct < CT; ++ct) {
@@ -309,18 +358,16 @@ __global__ __launch_bounds__(256, KV4_WAVES(HD, CT)) void kv4_attn_kernel(const 
           acc[ct][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, lo[ct], acc[ct][j], 0, 0, 0);
         }
       }
-#pragma unroll
-      for (int ct = 0; ct < CT; ++ct) asm volatile("" : "+v"(l[ct]), "+v"(cst[ct]));  // (their sums are not put off past the next loads)
-      __builtin_amdgcn_sched_barrier(0);
-      load_values();
       tile += 4;
+      from = from == S - 1 ? 0 : from + 1;
     }
     return true;
   };
   if (tile < tile1) {
-    ask_pages(tile);
-    load_keys(tile);
-    load_values();
+    ask_pages();
+#pragma unroll
+    for (int i = 0; i < S - 1; ++i)
+      if (ahead < tile1) issue();
   }
   while (tile < tile1) {
     if (needs_mask() ? run(std::true_type{}) : run(std::false_type{})) continue;
@@ -354,7 +401,7 @@ __global__ __launch_bounds__(256, KV4_WAVES(HD, CT)) void kv4_attn_kernel(const 
       s_c[w][ct * 16 + n16] = cst[ct];
     }
   }
-  __syncthreads();
+  __syncthreads();  // (the rings are read, nothing is in flight: their memory takes the outputs)
   const bool split = p.n_split > 1;
   const int oc = tid >> 4, och = (tid & 15) * (HC / 16);
 #pragma unroll
@@ -506,12 +553,19 @@ extern "C" int grove_kv4_attn(const grove_kv4_attn_params* p, void* stream) {
   const int64_t chunks = (cols + 16 * ct - 1) / (16 * ct);
   GROVE_CHECK(chunks * p->kv <= 65535, GROVE_E_SHAPE, "kv4_attn: too many new tokens in a request (%lld columns)", (long long)cols);
   const dim3 grid((unsigned)p->n_split, (unsigned)(chunks * p->kv), (unsigned)p->requests);
-#define LAUNCH(HD)                                                                                                                            \
-  if (ct == 1) hipLaunchKernelGGL((kv4_attn_kernel<HD, 1>), grid, dim3(256), 0, (hipStream_t)stream, *p, shift, vec_q, vec_o);                \
-  else if (ct == 2) hipLaunchKernelGGL((kv4_attn_kernel<HD, 2>), grid, dim3(256), 0, (hipStream_t)stream, *p, shift, vec_q, vec_o);           \
-  else hipLaunchKernelGGL((kv4_attn_kernel<HD < 256 ? HD : 128, 4>), grid, dim3(256), 0, (hipStream_t)stream, *p, shift, vec_q, vec_o)
+#define RUN(HD, CT)                                                                                                                  \
+  do {                                                                                                                               \
+    constexpr int lds = 4 * kv4_slots(HD, CT) * kv4_bytes(HD);                                                                       \
+    hipFuncSetAttribute((const void*)kv4_attn_kernel<HD, CT>, hipFuncAttributeMaxDynamicSharedMemorySize, lds);                      \
+    hipLaunchKernelGGL((kv4_attn_kernel<HD, CT>), grid, dim3(256), lds, (hipStream_t)stream, *p, shift, vec_q, vec_o);               \
+  } while (0)
+#define LAUNCH(HD)                       \
+  if (ct == 1) RUN(HD, 1);               \
+  else if (ct == 2) RUN(HD, 2);          \
+  else RUN((HD < 256 ? HD : 128), 4)
   KV4_HD(p->hd, LAUNCH)
 #undef LAUNCH
+#undef RUN
   GROVE_LAUNCH_CHECK();
   if (p->n_split > 1) {
     const int64_t units = (int64_t)p->rows * p->heads;
