@@ -94,11 +94,11 @@ __global__ __launch_bounds__(64) void kv4_read_kernel(const grove_kv4_read_param
 //     (hi + lo, 2^-17), the minimum's share sum P (m - 16 s) is one number per column.
 // Running maximum in log2 units, raised only where a score passes it by 8 (P <= 2^8 keeps its precision in fp32): most tiles skip the rescaling.
 // The tiles travel global -> LDS (LDS-DMA) into a ring of kv4_slots slots per wave: several tiles per wave are in flight without a register held
-// for them, and every lane takes back the bytes that it asked for (its K and V pieces side by side in lane order: no bank conflicts, and no
-// barrier, since a wave reads only its own ring). Waits are counted: a tile is kv4_ops vector memory operations.
+// for them. At hd 128 and 256 every lane takes back the bytes that it asked for, side by side in lane order: no bank conflicts. No barriers: a wave
+// reads only its own ring. Waits are counted: a tile is kv4_ops vector memory operations.
 constexpr int kv4_part(int hd) { return 64 * (hd / 8); }              // bytes of 16 keys' codes
 constexpr int kv4_bytes(int hd) { return 4 * kv4_part(hd) + 256; }    // of a tile: two parts of keys, two of values, scales
-constexpr int kv4_ops(int hd) { return 4 * (hd == 64 || hd == 256 ? 2 : 1) + 1; }
+constexpr int kv4_ops(int hd) { return hd / 32 + 1; }
 constexpr int kv4_slots(int hd, int ct) { return hd == 256 ? (ct == 1 ? 2 : 4) : hd == 128 ? (ct == 1 ? 3 : ct == 2 ? 4 : 6) : 4; }
 
 template <int HD>
@@ -123,10 +123,13 @@ __device__ __forceinline__ void ring_read(unsigned a, unsigned as, unsigned (&w)
                  : "=&v"(w[0][0]), "=&v"(w[1][0]), "=&v"(s[0]), "=&v"(s[1])
                  : "v"(a), "v"(as), "n"(O), "n"(O + 256), "n"(OS), "n"(OS + 64) : "memory");
   } else if constexpr (HD == 64) {
-    asm volatile("ds_read_b32 %0, %6 offset:%8\n\tds_read_b32 %1, %6 offset:%9\n\tds_read_b32 %2, %6 offset:%10\n\tds_read_b32 %3, %6 offset:%11\n\t"
-                 "ds_read_b128 %4, %7 offset:%12\n\tds_read_b128 %5, %7 offset:%13\n\ts_waitcnt lgkmcnt(0)"
-                 : "=&v"(w[0][0]), "=&v"(w[0][1]), "=&v"(w[1][0]), "=&v"(w[1][1]), "=&v"(s[0]), "=&v"(s[1])
-                 : "v"(a), "v"(as), "n"(O), "n"(O + 256), "n"(O + 512), "n"(O + 768), "n"(OS), "n"(OS + 64) : "memory");
+    u32x2_t x[2];
+    asm volatile("ds_read_b64 %0, %4 offset:%6\n\tds_read_b64 %1, %4 offset:%7\n\tds_read_b128 %2, %5 offset:%8\n\tds_read_b128 %3, %5 offset:%9\n\t"
+                 "s_waitcnt lgkmcnt(0)"
+                 : "=&v"(x[0]), "=&v"(x[1]), "=&v"(s[0]), "=&v"(s[1])
+                 : "v"(a), "v"(as), "n"(O), "n"(O + 512), "n"(OS), "n"(OS + 64) : "memory");
+#pragma unroll
+    for (int u = 0; u < 2; ++u) { w[u][0] = x[u][0]; w[u][1] = x[u][1]; }
   } else {
     constexpr int N = HD / 128;
     u32x4_t x[2][N];
@@ -177,6 +180,9 @@ __global__ __launch_bounds__(256, KV4_WAVES(HD, CT)) void kv4_attn_kernel(const 
   float(*s_o)[16][HC + 4] = (float(*)[16][HC + 4])smem;
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), n16 = lane & 15, h = lane >> 4;
   const int G = p.heads / p.kv, chunks = gridDim.y / p.kv, hk = blockIdx.y / chunks, cc = blockIdx.y - hk * chunks, b = blockIdx.z, sp = blockIdx.x;
+  typedef const __attribute__((address_space(4))) int* scalar_ints;  // scalar loads: of inputs that nothing writes meanwhile
+  const scalar_ints cu_q = (scalar_ints)(uintptr_t)p.cu_q;
+  const int q_lo = cu_q[b], q_hi = cu_q[b + 1], kv_len = ((scalar_ints)(uintptr_t)p.kv_len)[b];
   if (p.fresh && p.n_split == 1 && b == 0 && cc == 0) {  // a new result's rows of no request
     const int r0 = max(0, min(p.cu_q[0], p.rows)), r1 = max(r0, min(p.cu_q[p.requests], p.rows));
     for (int64_t e = tid; e < (int64_t)(r0 + p.rows - r1) * G * HD; e += 256) {
@@ -184,50 +190,62 @@ __global__ __launch_bounds__(256, KV4_WAVES(HD, CT)) void kv4_attn_kernel(const 
       ((bf16_raw*)p.out)[(r < r0 ? r : r1 + r - r0) * p.so_row + (int64_t)hk * G * HD + e % (G * HD)] = 0;
     }
   }
-  const int t0 = max(0, min(p.cu_q[b], p.rows)), t1 = max(t0, min(p.cu_q[b + 1], p.rows)), n = t1 - t0;
+  const int t0 = max(0, min(q_lo, p.rows)), t1 = max(t0, min(q_hi, p.rows)), n = t1 - t0;
   const int cols = min(n, p.max_q) * G, col0 = cc * 16 * CT;
   if (col0 >= cols) return;
   const int64_t room = (int64_t)p.max_pages << shift;
-  const int base = (int)min((int64_t)p.kv_len[b], room) - n + 1;  // token i sees base + i keys
+  const int base = (int)min((int64_t)kv_len, room) - n + 1;  // token i sees base + i keys
   const int seen_all = max(0, base + col0 / G), seen_any = max(0, base + (min(cols, col0 + 16 * CT) - 1) / G);
   const int tiles = (seen_any + 31) >> 5, per = (tiles + p.n_split - 1) / p.n_split, tile0 = sp * per, tile1 = min(tiles, tile0 + per);
 
-  bf16x8_t q[CT][NK];
-  float qs[CT], ref[CT], over[CT], l[CT], cst[CT];  // ref: taken off the scores; over: ref + 8, or -inf before the column's first key
-  int lim[CT];
-  const float a2 = p.alpha * 1.44269504088896340736f;
-#pragma unroll
-  for (int ct = 0; ct < CT; ++ct) {
-    const int c = col0 + ct * 16 + n16, i = c / G;
-    const bf16_raw* x = (const bf16_raw*)p.q + (t0 + i) * p.sq_row + (int64_t)(hk * G + c - i * G) * p.sq_head + 8 * h;
-    float sum = 0.f;
-#pragma unroll
-    for (int t = 0; t < NK; ++t) {
-      u32x4_t r = {0, 0, 0, 0};
-      if (c < cols) {
-        if (vec_q) r = *(const u32x4_t*)(x + 32 * t);
-        else
-          for (int e = 0; e < 4; ++e) r[e] = x[32 * t + 2 * e] | ((unsigned)x[32 * t + 2 * e + 1] << 16);
-      }
-      q[ct][t] = __builtin_bit_cast(bf16x8_t, r);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) sum += bf_lo(r[e]) + bf_hi(r[e]);
-    }
-    sum += __shfl_xor(sum, 16, 64);
-    sum += __shfl_xor(sum, 32, 64);
-    qs[ct] = sum * a2;
-    lim[ct] = c < cols ? base + i : 0;
-    over[ct] = NEG;
-    ref[ct] = l[ct] = cst[ct] = 0.f;
-  }
   f32x4_t acc[CT][NJ];
 #pragma unroll
   for (int ct = 0; ct < CT; ++ct)
 #pragma unroll
     for (int j = 0; j < NJ; ++j) acc[ct][j] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
 
+  // the columns' queries: asked for after the page numbers and before the first tiles, used when those are on their way
+  bf16x8_t q[CT][NK];
+  auto ask_q = [&]() {
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+      const int c = col0 + ct * 16 + n16, i = c / G;
+      const bf16_raw* x = (const bf16_raw*)p.q + (t0 + i) * p.sq_row + (int64_t)(hk * G + c - i * G) * p.sq_head + 8 * h;
+#pragma unroll
+      for (int t = 0; t < NK; ++t) {
+        u32x4_t r = {0, 0, 0, 0};
+        if (c < cols) {
+          if (vec_q) r = *(const u32x4_t*)(x + 32 * t);
+          else
+            for (int e = 0; e < 4; ++e) r[e] = x[32 * t + 2 * e] | ((unsigned)x[32 * t + 2 * e + 1] << 16);
+        }
+        q[ct][t] = __builtin_bit_cast(bf16x8_t, r);
+      }
+    }
+  };
+  float qs[CT], ref[CT], over[CT], l[CT], cst[CT];  // ref: taken off the scores; over: ref + 8, or -inf before the column's first key
+  int lim[CT];
+  const float a2 = p.alpha * 1.44269504088896340736f;
+  auto use_q = [&]() {
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+      const int c = col0 + ct * 16 + n16, i = c / G;
+      float sum = 0.f;
+#pragma unroll
+      for (int t = 0; t < NK; ++t) {
+        const u32x4_t r = __builtin_bit_cast(u32x4_t, q[ct][t]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum += bf_lo(r[e]) + bf_hi(r[e]);
+      }
+      sum += __shfl_xor(sum, 16, 64);
+      sum += __shfl_xor(sum, 32, 64);
+      qs[ct] = sum * a2;
+      lim[ct] = c < cols ? base + i : 0;
+      over[ct] = NEG;
+      ref[ct] = l[ct] = cst[ct] = 0.f;
+    }
+  };
   // page numbers by scalar loads (the constant address space), asked for one tile ahead of their use
-  typedef const __attribute__((address_space(4))) int* scalar_ints;
   const scalar_ints row = (scalar_ints)(uintptr_t)(p.table + b * p.ld_table);
   const int P = 1 << shift;
   const int64_t page_rows = (int64_t)2 * p.kv << shift, v_rows = (int64_t)p.kv << shift;  // cache rows of a page, and from its keys to its values
@@ -252,16 +270,21 @@ __global__ __launch_bounds__(256, KV4_WAVES(HD, CT)) void kv4_attn_kernel(const 
       const bool ok = (ask[u] >= 0) & (ask[u] < p.pages);
       miss |= ok ? 0u : 1u << u;
       at[u] = (int64_t)(ok ? ask[u] : 0) * page_rows + ((ahead * 32 + 16 * u) & (P - 1));
-      const unsigned char* kp = codes + at[u] * (HD / 2) + k_off;
-      const unsigned char* vp = codes + (at[u] + v_rows) * (HD / 2) + v_off;
-      char* kl = slot + u * PART;
-      if constexpr (HD >= 128) {
+    }
+    if constexpr (HD >= 128) {  // a lane's pieces for itself: 16 bytes of each part's keys and values
 #pragma unroll
-        for (int i = 0; i < HD / 128; ++i) { dma16(kp + 16 * i, kl + 1024 * i); dma16(vp + 16 * i, kl + 2 * PART + 1024 * i); }
-      } else {
+      for (int u = 0; u < 2; ++u)
 #pragma unroll
-        for (int i = 0; i < HD / 32; ++i) { dma4(kp + 4 * i, kl + 256 * i); dma4(vp + 4 * i, kl + 2 * PART + 256 * i); }
-      }
+        for (int i = 0; i < HD / 128; ++i) {
+          dma16(codes + at[u] * (HD / 2) + k_off + 16 * i, slot + u * PART + 1024 * i);
+          dma16(codes + (at[u] + v_rows) * (HD / 2) + v_off + 16 * i, slot + (2 + u) * PART + 1024 * i);
+        }
+    } else if constexpr (HD == 64) {  // both parts' 512 bytes in one load, in memory's order
+      const int64_t mine = lane < 32 ? at[0] : at[1];
+      dma16(codes + mine * 32 + (lane & 31) * 16, slot);
+      dma16(codes + (mine + v_rows) * 32 + (lane & 31) * 16, slot + 2 * PART);
+    } else {  // all four parts' 256 bytes
+      dma16(codes + (((h & 1) ? at[1] : at[0]) + (h >= 2 ? v_rows : 0)) * 16 + n16 * 16, slot);
     }
     dma4(scales + ((h & 1) ? at[1] : at[0]) + (h >= 2 ? v_rows : 0) + n16, slot + 4 * PART);  // keys' parts 0, 1, values' parts 0, 1
     bad = (bad & ~(3u << (2 * to))) | miss << (2 * to);
@@ -283,8 +306,9 @@ __global__ __launch_bounds__(256, KV4_WAVES(HD, CT)) void kv4_attn_kernel(const 
       auto sees = [&](int ct, int u, int i) { return (tile * 32 + 16 * u + 4 * h + i < lim[ct]) & ((bad >> (2 * from + u) & 1) == 0); };
       if (ahead - tile == 4 * (S - 1)) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(OPS * (S - 2)) : "memory");  // the tiles behind this one may be on their way
       else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");                                                  // the last ones
-      const unsigned slot = ring_at + from * BYTES, at_codes = slot + lane * (HD < 128 ? 4 : 16), at_scales = slot + 16 * h;
-      ring_read<HD, 0, 4 * PART>(at_codes, at_scales, T.k, T.ks);
+      const unsigned slot = ring_at + from * BYTES, at_scales = slot + 16 * h;
+      const unsigned at_keys = slot + (HD < 128 ? n16 * (HD / 2) + h * (HD / 8) : lane * 16), at_values = slot + lane * (HD < 128 ? HD / 8 : 16);
+      ring_read<HD, 0, 4 * PART>(at_keys, at_scales, T.k, T.ks);
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         __builtin_amdgcn_sched_barrier(0);  // one part's operands at a time: unpacked all at once they would take the registers of a third wave
@@ -315,7 +339,7 @@ __global__ __launch_bounds__(256, KV4_WAVES(HD, CT)) void kv4_attn_kernel(const 
       }
       if (__any(grow)) return false;
       if (ahead < tile1) issue();
-      ring_read<HD, 2 * PART, 4 * PART + 128>(at_codes, at_scales, T.v, T.vs);
+      ring_read<HD, 2 * PART, 4 * PART + 128>(at_values, at_scales, T.v, T.vs);
       bf16x8_t hi[CT], lo[CT];
 #pragma unroll
       for (int ct = 0; ct < CT; ++ct) {
@@ -363,12 +387,12 @@ __global__ __launch_bounds__(256, KV4_WAVES(HD, CT)) void kv4_attn_kernel(const 
     }
     return true;
   };
-  if (tile < tile1) {
-    ask_pages();
+  if (tile < tile1) ask_pages();
+  ask_q();
 #pragma unroll
-    for (int i = 0; i < S - 1; ++i)
-      if (ahead < tile1) issue();
-  }
+  for (int i = 0; i < S - 1; ++i)
+    if (ahead < tile1) issue();
+  use_q();
   while (tile < tile1) {
     if (needs_mask() ? run(std::true_type{}) : run(std::false_type{})) continue;
 #pragma unroll
@@ -457,12 +481,14 @@ __global__ __launch_bounds__(256, KV4_WAVES(HD, CT)) void kv4_attn_kernel(const 
   }
 }
 
-// Joins the partial results of the splits: one wave per (row, query head).
-template <int HD>
+// Joins the partial results of at most 64 splits: a lane per split for the weights, then WAVES waves over the splits of one (row, query head), eight
+// partial outputs in flight. One wave each where the splits are few.
+template <int HD, int WAVES>
 __global__ __launch_bounds__(256) void kv4_join_kernel(const grove_kv4_attn_params p) {
   constexpr int NC = HD < 64 ? 1 : HD / 64;
-  const int lane = threadIdx.x & 63, S = p.n_split;
-  const int64_t unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  __shared__ float s_o[4][HD];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, S = p.n_split;
+  const int64_t unit = WAVES == 1 ? (int64_t)blockIdx.x * 4 + w : (int64_t)blockIdx.x;
   if (unit >= (int64_t)p.rows * p.heads) return;
   const int row = (int)(unit / p.heads), head = (int)(unit - (int64_t)row * p.heads);
   const bool mine = row >= p.cu_q[0] && row < p.cu_q[p.requests];
@@ -471,19 +497,38 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(const grove_kv4_attn_para
   float o[NC] = {}, L = 0.f;
   if (mine) {
     const float* ml = p.partial + (int64_t)p.rows * p.heads * S * HD + unit * S * 2;
-    const float* part = p.partial + unit * S * HD;
-    float M = NEG;
-    for (int s = lane; s < S; s += 64) M = fmaxf(M, ml[2 * s]);
-    M = wave_max(M);
-    for (int s = 0; s < S; ++s) {
-      const float ms = ml[2 * s], ls = ml[2 * s + 1];
-      if (ls == 0.f) continue;  // a split without keys wrote no output
-      const float f = ms == NEG ? 0.f : __builtin_amdgcn_exp2f(ms - M);
-      L += f * ls;
+    const float* part = p.partial + unit * S * HD + min(lane, HD - 1);
+    float ms = NEG, ls = 0.f;
+    if (lane < S) { ms = ml[2 * lane]; ls = ml[2 * lane + 1]; }
+    const bool live = ls != 0.f;  // a split without keys wrote no output
+    const float M = wave_max(live ? ms : NEG), f = !live || ms == NEG ? 0.f : __builtin_amdgcn_exp2f(ms - M);
+    L = wave_sum(live ? f * ls : 0.f);
+    const unsigned long long alive = __ballot(live);
+    for (int s0 = WAVES == 1 ? 0 : w; s0 < S; s0 += 8 * WAVES) {
+      float x[8][NC];
 #pragma unroll
-      for (int i = 0; i < NC; ++i)
-        if (HD >= 64 || lane < HD) o[i] += f * part[(int64_t)s * HD + lane + 64 * i];
+      for (int k = 0; k < 8; ++k)
+#pragma unroll
+        for (int i = 0; i < NC; ++i) x[k][i] = part[(int64_t)min(s0 + k * WAVES, S - 1) * HD + 64 * i];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const int s = s0 + k * WAVES;
+        const float fs = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f), min(s, 63)));
+        if (s < S && (alive >> s & 1))
+#pragma unroll
+          for (int i = 0; i < NC; ++i) o[i] += fs * x[k][i];
+      }
     }
+  }
+  if constexpr (WAVES > 1) {
+#pragma unroll
+    for (int i = 0; i < NC; ++i)
+      if (HD >= 64 || lane < HD) s_o[w][lane + 64 * i] = o[i];
+    __syncthreads();
+    if (w > 0) return;
+#pragma unroll
+    for (int i = 0; i < NC; ++i)
+      if (HD >= 64 || lane < HD) o[i] = (s_o[0][lane + 64 * i] + s_o[1][lane + 64 * i]) + (s_o[2][lane + 64 * i] + s_o[3][lane + 64 * i]);
   }
   const bool some = L > 0.f || L != L;
 #pragma unroll
@@ -543,7 +588,7 @@ extern "C" int grove_kv4_attn(const grove_kv4_attn_params* p, void* stream) {
   if (p->rows == 0 || p->requests == 0 || p->max_q == 0) return GROVE_OK;
   GROVE_CHECK(p->q && p->codes && p->scales && p->table && p->kv_len && p->cu_q && p->out, GROVE_E_SHAPE, "kv4_attn: null pointer");
   GROVE_CHECK(((uintptr_t)p->codes & 15) == 0 && ((uintptr_t)p->scales & 15) == 0, GROVE_E_ALIGN, "kv4_attn: the cache must be 16-byte aligned");
-  GROVE_CHECK(p->n_split >= 1 && p->n_split <= 65535 && (p->n_split == 1 || p->partial), GROVE_E_WORKSPACE, "kv4_attn: a split needs its workspace");
+  GROVE_CHECK(p->n_split >= 1 && p->n_split <= 64 && (p->n_split == 1 || p->partial), GROVE_E_WORKSPACE, "kv4_attn: 1 to 64 splits, more than one with a workspace");
   GROVE_CHECK((int64_t)p->max_pages * p->page <= 0x7fffffff, GROVE_E_SHAPE, "kv4_attn: the table holds more than 2^31 tokens");
   const int shift = __builtin_ctz((unsigned)p->page);
   const int vec_q = ((uintptr_t)p->q & 15) == 0 && p->sq_row % 8 == 0 && p->sq_head % 8 == 0, vec_o = ((uintptr_t)p->out & 15) == 0 && p->so_row % 8 == 0;
@@ -569,8 +614,10 @@ extern "C" int grove_kv4_attn(const grove_kv4_attn_params* p, void* stream) {
   GROVE_LAUNCH_CHECK();
   if (p->n_split > 1) {
     const int64_t units = (int64_t)p->rows * p->heads;
-    GROVE_CHECK((units + 3) / 4 <= 0x7fffffff, GROVE_E_SHAPE, "kv4_attn: too many rows");
-#define LAUNCH(HD) hipLaunchKernelGGL(kv4_join_kernel<HD>, dim3((unsigned)((units + 3) / 4)), dim3(256), 0, (hipStream_t)stream, *p)
+    GROVE_CHECK(units <= 0x7fffffff, GROVE_E_SHAPE, "kv4_attn: too many rows");
+#define LAUNCH(HD)                                                                                                                                  \
+  if (p->n_split > 8) hipLaunchKernelGGL((kv4_join_kernel<HD, 4>), dim3((unsigned)units), dim3(256), 0, (hipStream_t)stream, *p);                   \
+  else hipLaunchKernelGGL((kv4_join_kernel<HD, 1>), dim3((unsigned)((units + 3) / 4)), dim3(256), 0, (hipStream_t)stream, *p)
     KV4_HD(p->hd, LAUNCH)
 #undef LAUNCH
     GROVE_LAUNCH_CHECK();

@@ -711,7 +711,7 @@ int grove_kv4_read(const grove_kv4_read_params* p, void* stream);
  *   out[r] = softmax(alpha * q[r] . K[t]) V, fp32 throughout; 0 where it sees none.
  * Keys whose table entry is outside [0, pages) are not seen. kv_len is cut to max_pages * page. Rows of no request are left as they
  * were. n must not pass max_q. Rows of the cache that no query sees may hold anything.
- * n_split > 1: a request's keys are dealt to n_split blocks, whose partial results lie in `partial`, f32 [rows * heads * n_split *
+ * n_split > 1 (at most 64): a request's keys are dealt to n_split blocks, whose partial results lie in `partial`, f32 [rows * heads * n_split *
  * (hd + 2)], and are joined by a second launch. Otherwise `partial` may be NULL. */
 typedef struct grove_kv4_attn_params {
   const void* q;
