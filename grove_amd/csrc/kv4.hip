@@ -92,7 +92,6 @@ __global__ __launch_bounds__(64) void kv4_read_kernel(const grove_kv4_read_param
 //   O^T[c, col] += sum_key V[key, c] (P s)[key, col]   A = channels (16) x 32 keys, B = the scores' own registers: the accumulator of S^T holds keys
 //     4 h + i of either part in lane (col, h), and the values' four-token order gives the A operand the same keys. P s goes in as two bf16 parts
 //     (hi + lo, 2^-17), the minimum's share sum P (m - 16 s) is one number per column.
-// Running maximum in log2 units, raised only where a score passes it by 8 (P <= 2^8 keeps its precision in fp32): most tiles skip the rescaling.
 // The tiles travel global -> LDS (LDS-DMA) into a ring of kv4_slots slots per wave: several tiles per wave are in flight without a register held
 // for them. At hd 128 and 256 every lane takes back the bytes that it asked for, side by side in lane order: no bank conflicts. No barriers: a wave
 // reads only its own ring. Waits are counted: a tile is kv4_ops vector memory operations.
@@ -198,12 +197,6 @@ __global__ __launch_bounds__(256, KV4_WAVES(HD, CT)) void kv4_attn_kernel(const 
   const int seen_all = max(0, base + col0 / G), seen_any = max(0, base + (min(cols, col0 + 16 * CT) - 1) / G);
   const int tiles = (seen_any + 31) >> 5, per = (tiles + p.n_split - 1) / p.n_split, tile0 = sp * per, tile1 = min(tiles, tile0 + per);
 
-  f32x4_t acc[CT][NJ];
-#pragma unroll
-  for (int ct = 0; ct < CT; ++ct)
-#pragma unroll
-    for (int j = 0; j < NJ; ++j) acc[ct][j] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
-
   // the columns' queries: asked for after the page numbers and before the first tiles, used when those are on their way
   bf16x8_t q[CT][NK];
   auto ask_q = [&]() {
@@ -223,7 +216,7 @@ __global__ __launch_bounds__(256, KV4_WAVES(HD, CT)) void kv4_attn_kernel(const 
       }
     }
   };
-  float qs[CT], ref[CT], over[CT], l[CT], cst[CT];  // ref: taken off the scores; over: ref + 8, or -inf before the column's first key
+  float qs[CT], ref[CT], over[CT], l[CT], cst[CT];  // ref: taken off the scores; over: ref + 24, or -inf before the column's first key
   int lim[CT];
   const float a2 = p.alpha * 1.44269504088896340736f;
   auto use_q = [&]() {
@@ -242,7 +235,7 @@ __global__ __launch_bounds__(256, KV4_WAVES(HD, CT)) void kv4_attn_kernel(const 
       qs[ct] = sum * a2;
       lim[ct] = c < cols ? base + i : 0;
       over[ct] = NEG;
-      ref[ct] = l[ct] = cst[ct] = 0.f;
+      ref[ct] = 0.f;
     }
   };
   // page numbers by scalar loads (the constant address space), asked for one tile ahead of their use
@@ -255,7 +248,7 @@ __global__ __launch_bounds__(256, KV4_WAVES(HD, CT)) void kv4_attn_kernel(const 
   const int k_off = n16 * (HD / 2) + h * (HD / 8), v_off = h * (2 * HD) + n16 * (HD / 8);
   char* ring = smem + w * S * BYTES;
   const unsigned ring_at = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)ring;
-  int ask[2], ahead = tile0 + w, to = 0;  // the tile to be asked for next, and its slot
+  int ask[2], ahead, to;  // the tile to be asked for next, and its slot
   unsigned bad = 0;                       // two bits a slot: a part whose page is not one of the cache (its keys are masked, its loads go to page 0)
   auto ask_pages = [&]() {
 #pragma unroll
@@ -294,16 +287,14 @@ __global__ __launch_bounds__(256, KV4_WAVES(HD, CT)) void kv4_attn_kernel(const 
   };
   kv4_tile<HD> T;
 
-  // The tiles are run in two loops, with masks and without, and both are left where a score passes its column's maximum by 8: the accumulators are
-  // then rescaled between the loops and the tile is taken again. Branches around the rescaling or the masks inside one loop cost a copy of every
-  // accumulator per tile, and their merged paths a wait for the loads in flight.
-  int tile = tile0 + w, from = 0;
+  // A wave's tiles. A column's reference is the maximum of its first keys; the accumulators are never rescaled: where a later score passes it by 24
+  // (P <= 2^24 loses nothing in fp32) the wave starts again with that score's reference. Scores that far above a wave's first 32 keys' are rare, and
+  // rescaling in the loop costs a second set of registers for the accumulators (57 of them at CT = 2) or a copy of each per tile.
+  f32x4_t acc[CT][NJ];
+  int tile, from;
   float z[CT][8], top[CT];
-  auto needs_mask = [&]() { return ((tile + 1) * 32 > seen_all) | ((bad >> (2 * from) & 3) != 0); };
-  auto run = [&](auto masked) -> bool {  // false: left for a rescaling
-    constexpr bool MASK = decltype(masked)::value;
-    while ((tile < tile1) & (needs_mask() == MASK)) {
-      auto sees = [&](int ct, int u, int i) { return (tile * 32 + 16 * u + 4 * h + i < lim[ct]) & ((bad >> (2 * from + u) & 1) == 0); };
+  auto run = [&]() -> bool {  // false: left at a tile, with its scores, for new references
+    while (tile < tile1) {
       if (ahead - tile == 4 * (S - 1)) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(OPS * (S - 2)) : "memory");  // the tiles behind this one may be on their way
       else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");                                                  // the last ones
       const unsigned slot = ring_at + from * BYTES, at_scales = slot + 16 * h;
@@ -323,11 +314,18 @@ __global__ __launch_bounds__(256, KV4_WAVES(HD, CT)) void kv4_attn_kernel(const 
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const float s = bf_lo(T.ks[u][i]), mn = bf_hi(T.ks[u][i]);
-            float v = fmaf(raw[i], a2 * s, fmaf(-16.f, s, mn) * qs[ct]);
-            if constexpr (MASK) v = sees(ct, u, i) ? v : NEG;
-            z[ct][4 * u + i] = v;
+            z[ct][4 * u + i] = fmaf(raw[i], a2 * s, fmaf(-16.f, s, mn) * qs[ct]);
           }
         }
+      }
+      const unsigned miss = bad >> (2 * from) & 3;
+      const bool masked = ((tile + 1) * 32 > seen_all) | (miss != 0);
+      auto sees = [&](int ct, int i) { return (tile * 32 + 16 * (i >> 2) + 4 * h + (i & 3) < lim[ct]) & ((miss >> (i >> 2) & 1) == 0); };
+      if (masked) {
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) z[ct][i] = sees(ct, i) ? z[ct][i] : NEG;
       }
       bool grow = false;
 #pragma unroll
@@ -340,6 +338,16 @@ __global__ __launch_bounds__(256, KV4_WAVES(HD, CT)) void kv4_attn_kernel(const 
       if (__any(grow)) return false;
       if (ahead < tile1) issue();
       ring_read<HD, 2 * PART, 4 * PART + 128>(at_values, at_scales, T.v, T.vs);
+      if (masked) {  // 0 times a scale that is no number would reach the columns that do not see its row: it goes, and those that see it become NaN
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const unsigned sm = T.vs[i >> 2][i & 3];
+          const bool odd = ((sm & 0x7f80u) == 0x7f80u) | ((sm & 0x7f800000u) == 0x7f800000u);
+#pragma unroll
+          for (int ct = 0; ct < CT; ++ct) l[ct] = odd & sees(ct, i) ? NAN : l[ct];
+          T.vs[i >> 2][i & 3] = odd ? 0u : sm;
+        }
+      }
       bf16x8_t hi[CT], lo[CT];
 #pragma unroll
       for (int ct = 0; ct < CT; ++ct) {
@@ -353,10 +361,7 @@ __global__ __launch_bounds__(256, KV4_WAVES(HD, CT)) void kv4_attn_kernel(const 
             const float s = bf_lo(T.vs[u][i]), mn = fmaf(-16.f, s, bf_hi(T.vs[u][i]));
             l[ct] += e;
             ps[i] = e * s;
-            if constexpr (MASK) {  // an unseen row's scale may be anything
-              ps[i] = sees(ct, u, i) ? ps[i] : 0.f;
-              cst[ct] += sees(ct, u, i) ? e * mn : 0.f;
-            } else cst[ct] = fmaf(e, mn, cst[ct]);
+            cst[ct] = fmaf(e, mn, cst[ct]);
           }
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
@@ -387,30 +392,42 @@ __global__ __launch_bounds__(256, KV4_WAVES(HD, CT)) void kv4_attn_kernel(const 
     }
     return true;
   };
-  if (tile < tile1) ask_pages();
-  ask_q();
+  bool fresh_q = true, again;
+  do {
+    again = false;
+    tile = ahead = tile0 + w;
+    to = from = 0;
+    bad = 0;
+    if (tile < tile1) ask_pages();
+    if (fresh_q) ask_q();
 #pragma unroll
-  for (int i = 0; i < S - 1; ++i)
-    if (ahead < tile1) issue();
-  use_q();
-  while (tile < tile1) {
-    if (needs_mask() ? run(std::true_type{}) : run(std::false_type{})) continue;
+    for (int i = 0; i < S - 1; ++i)
+      if (ahead < tile1) issue();
+    if (fresh_q) use_q();
+    fresh_q = false;
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
-      float t = fmaxf(top[ct], __shfl_xor(top[ct], 16, 64));
-      t = fmaxf(t, __shfl_xor(t, 32, 64));
-      const bool up = t > over[ct];
-      const float f = up && over[ct] != NEG ? __builtin_amdgcn_exp2f(ref[ct] - t) : 1.f;  // (before the first key there is nothing to rescale)
-      if (up) {
-        ref[ct] = t;
-        over[ct] = t + 8.f;
-      }
-      l[ct] *= f;
-      cst[ct] *= f;
+      l[ct] = cst[ct] = 0.f;
 #pragma unroll
-      for (int j = 0; j < NJ; ++j) acc[ct][j] *= f;
+      for (int j = 0; j < NJ; ++j) acc[ct][j] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
     }
-  }
+    while (!run()) {
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) {
+        float t = fmaxf(top[ct], __shfl_xor(top[ct], 16, 64));
+        t = fmaxf(t, __shfl_xor(t, 32, 64));
+        const bool up = t > over[ct];
+        again |= up && over[ct] != NEG;  // (a column's first keys leave nothing to do again)
+        ref[ct] = up ? t : ref[ct];
+        over[ct] = up ? t + 24.f : over[ct];
+      }
+      again = __any(again);
+      if (again) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the tiles in flight land before their slots are asked for again
+        break;
+      }
+    }
+  } while (again);
 
   // the four waves' results: one maximum per column, the outputs through LDS
 #pragma unroll

@@ -410,6 +410,27 @@ def test_attn_peaked_and_large_scores(dev):
     check_attn(dev, [200], [1], 4, 4, 64, 16, spread=1e-3)
 
 
+@pytest.mark.parametrize("H,kv,new,hd", [(4, 2, 1, 64), (8, 1, 4, 128), (16, 2, 8, 64), (4, 4, 3, 256)])
+def test_attn_climbing_scores(dev, H, kv, new, hd):
+    """Keys that outgrow everything before them again and again: the references of the running softmax have to follow."""
+    from grove_amd import ops
+    L, P = 700, 16
+    c = Paged(dev, [L, 40], kv, hd, P, seed=71)
+    g = gen(72)
+    q = (torch.randn(2 * new, H, hd, generator=g) + 1.0).to(bf16)
+    k = torch.randn(L, kv, hd, generator=g) * 0.05 + (torch.arange(L) ** 2 / 2000.0)[:, None, None] * (1 + torch.rand(kv, hd, generator=g)) / hd ** 0.5
+    v = torch.randn(L, kv, hd, generator=g)
+    ops.kv4_append(k.to(bf16).to(dev), v.to(bf16).to(dev), c.cache, c.slots[:L])
+    kk, vv = (t.cpu().to(f64) for t in ops.kv4_read(c.cache, c.slots, f32))
+    c.k, c.v = kk.split([L, 40]), vv.split([L, 40])
+    step = [(t.amax(-1) - t.amin(-1)) / 15 for t in (kk, vv)]
+    c.size = [float(31 * s.max() + t.abs().max()) for s, t in zip(step, (kk, vv))]
+    cu = torch.tensor([0, new, 2 * new], dtype=i32, device=dev)
+    out = ops.kv4_attn(q.to(dev), c.cache, c.table, torch.tensor([L, 40], dtype=i32, device=dev), cu, new, 1.0)
+    ref, tol = c.ref(q, [new, new], 1.0)
+    within(out, ref, tol)
+
+
 def test_attn_single_key_is_its_value(dev):
     c, q, cu, kv_len, out = check_attn(dev, [1, 1], [1, 1], 4, 2, 128, 16)
     v = torch.stack([c.v[b][0].repeat_interleave(2, 0) for b in range(2)]).flatten(1)
