@@ -1434,10 +1434,15 @@ def kv4_read(cache, slots, out_dtype=bf16):
     return k, v
 
 
-def _kv4_split(pairs, max_len, cols):
-    """Blocks to which a request's keys are dealt."""
-    blocks = pairs * max(1, -(-cols // 64))
-    return max(1, min(64, max_len // 512, 2048 // blocks))
+def _kv4_split(pairs, max_len, cols, hd):
+    """Blocks to which the keys of a (request, key / value head) pair are dealt. A CU streams some 22 GB/s whatever it has in flight, so the 256 of
+    them are to be filled as soon as a block's four waves have three tiles of 32 keys (32 pairs of 703 keys: 10.6 us in one block each, 8.6 in
+    eight, 10 in sixteen); beyond that ragged lengths want some 2048 blocks as long as a block keeps 1024 keys (256 pairs of up to 32768 keys: 263
+    us in one block each, 128 in 8, 187 in 64), or 2048 per tile of 16 columns where there are several (512 pairs of up to 4096 keys under 32
+    columns: 70 us in one block each, 74 in 2, 101 in 8): behind that a block's start and its partial results count."""
+    ct = 1 if cols <= 16 else 2 if cols <= 32 or hd == 256 else 4
+    pairs *= max(1, -(-cols // (16 * ct)))
+    return max(1, min(64, max(min(256 // pairs, max_len // 96), min(2048 // pairs, max_len // (1024 if ct == 1 else 2048 * ct)))))
 
 
 def kv4_attn(q, cache, table, kv_len, cu_q, max_q, alpha, *, max_len=None, out=None):
@@ -1474,7 +1479,7 @@ def kv4_attn(q, cache, table, kv_len, cu_q, max_q, alpha, *, max_len=None, out=N
         if not all(_apart(out, t) for t in (q, codes, scales, table, kv_len, cu_q)):
             _refuse(what, "out overlaps an input")
         orow = out.stride(0)
-    n_split = _kv4_split(B * kv, most * P if max_len is None else max_len, max_q * (heads // kv))
+    n_split = _kv4_split(B * kv, most * P if max_len is None else max_len, min(max_q, rows) * (heads // kv), hd)
     # the joined splits' workspace: from the allocator at every call, so that calls on other streams and captured graphs have their own
     partial = torch.empty(rows * heads * n_split * (hd + 2), dtype=torch.float32, device=q.device) if n_split > 1 else None
     p = _lib.Kv4AttnParams(q.data_ptr(), codes.data_ptr(), scales.data_ptr(), table.data_ptr(), kv_len.data_ptr(), cu_q.data_ptr(), out.data_ptr(),
