@@ -4,82 +4,180 @@
 
 namespace {
 
-// Where channel c of the row `r` of a page is held: the byte within the (page, head) plane, and which nibble of it.
-template <int HD>
-__device__ __forceinline__ int key_byte(int r, int c, int& hi) {
-  const int t = c >> 5, h = (c >> 3) & 3, i = c & 7, nib = (i & 1) * 4 + (i >> 1);
-  hi = nib & 1;
-  return r * (HD / 2) + (h * (HD / 32) + t) * 4 + (nib >> 1);
-}
-template <int HD>
-__device__ __forceinline__ int value_byte(int r, int c, int& hi) {
-  const int tp = (r >> 1) & 1, par = r & 1, j = c >> 4, m = c & 15;
-  hi = j & 1;
-  const int quad = (r >> 2) * (2 * HD) + m * (HD / 8);
-  if constexpr (HD == 32) return quad + par * 2 + tp;
-  return quad + ((j >> 2) * 2 + tp) * 4 + par * 2 + ((j >> 1) & 1);
-}
-
-__device__ __forceinline__ bool slot_of(const int* slots, int row, int page, int pages, int& pg, int& at) {
-  const int s = slots[row];
+__device__ __forceinline__ bool slot_of(const int* slots, int row, int rows, int page, int pages, int& pg, int& at) {
+  const int s = row < rows ? slots[row] : -1;
   if (s < 0 || s >= (int64_t)pages * page) return false;
   pg = s / page;
   at = s - pg * page;
   return true;
 }
 
-// One wave per (row, head, keys or values).
-template <int HD>
-__global__ __launch_bounds__(64) void kv4_append_kernel(const grove_kv4_append_params p) {
-  __shared__ unsigned char code[HD];
-  const int lane = threadIdx.x, row = blockIdx.x, head = blockIdx.y, which = blockIdx.z;
-  int pg, at;
-  if (!slot_of(p.slots, row, p.page, p.pages, pg, at)) return;
-  const bf16_raw* x = which ? (const bf16_raw*)p.v + row * p.sv_row + head * p.sv_head : (const bf16_raw*)p.k + row * p.sk_row + head * p.sk_head;
-  float v[(HD + 63) / 64], lo = INFINITY, hi = -INFINITY;
+// ---------------------------------------------------------------- into the pages and out of them
+// HD / 8 lanes take one row of one head, 8 channels (16 bytes) each, so a wave holds 512 / HD consecutive rows: of a key row a lane's channels are one
+// word of the cache, of a value row one nibble of eight places, and four lanes exchange bytes to have all the nibbles of two places each. Bound by
+// memory for many rows, by the chain slot -> row -> page for few.
+
+// lane g's word holds the nibbles of channels 8 g + 0..7 (g = 2 j + half of the 16 places): a 4 x 4 transpose of bytes over the lanes j = 4 jq + 0..3
+__device__ __forceinline__ unsigned byte_transpose(unsigned w, int g) {
+  unsigned t = __shfl_xor(w, 2, 64);
+  w = (g & 2) ? __builtin_amdgcn_perm(t, w, 0x03070105) : __builtin_amdgcn_perm(t, w, 0x06020400);
+  t = __shfl_xor(w, 4, 64);
+  return (g & 4) ? __builtin_amdgcn_perm(t, w, 0x03020706) : __builtin_amdgcn_perm(t, w, 0x05040100);
+}
+__device__ __forceinline__ unsigned low_nibbles(unsigned w) {  // the low nibbles of the four bytes side by side
+  w &= 0x0f0f0f0fu;
+  w = (w | w >> 4) & 0x00ff00ffu;
+  return (w | w >> 8) & 0xffffu;
+}
+__device__ __forceinline__ unsigned spread_nibbles(unsigned w) {  // and back
+  w = (w | w << 8) & 0x00ff00ffu;
+  return (w | w << 4) & 0x0f0f0f0fu;
+}
+
+// The eight codes of a lane, nibble i = channel i; and the row's scale and minimum. G lanes share the row.
+template <int G>
+__device__ __forceinline__ unsigned quantise(const u32x4_t x, unsigned& scale_min) {
+  float v[8], lo, hi;
   bool bad = false;
-  for (int i = 0, c = lane; c < HD; c += 64, ++i) {
-    v[i] = bf2f(x[c]);
-    bad |= !(fabsf(v[i]) < INFINITY);
-    lo = fminf(lo, v[i]);
-    hi = fmaxf(hi, v[i]);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    v[2 * i] = bf_lo(x[i]);
+    v[2 * i + 1] = bf_hi(x[i]);
+    bad |= ((x[i] & 0x7f80u) == 0x7f80u) | ((x[i] & 0x7f800000u) == 0x7f800000u);
   }
-  lo = -wave_max(-lo);
-  hi = wave_max(hi);
+  lo = hi = v[0];
+#pragma unroll
+  for (int i = 1; i < 8; ++i) { lo = fminf(lo, v[i]); hi = fmaxf(hi, v[i]); }
+  int any = bad;
+#pragma unroll
+  for (int o = 1; o < G; o <<= 1) {
+    lo = fminf(lo, __shfl_xor(lo, o, 64));
+    hi = fmaxf(hi, __shfl_xor(hi, o, 64));
+    any |= __shfl_xor(any, o, 64);
+  }
   const float span = hi - lo;
-  bad = __any(bad) || !(span < INFINITY);
-  bf16_raw sb = span < 0x1p-100f ? 0 : f2bf(span / 15.f), mb = f2bf(lo);
-  if (bad) sb = mb = 0x7fc0;
-  const float s = bf2f(sb);
-  for (int i = 0, c = lane; c < HD; c += 64, ++i)
-    code[c] = (bad || s == 0.f) ? 0 : (unsigned char)fminf(fmaxf(rintf((v[i] - lo) / s), 0.f), 15.f);
-  __syncthreads();
-  const int64_t plane = ((int64_t)pg * 2 + which) * p.kv + head;
-  unsigned char* out = (unsigned char*)p.codes + plane * p.page * (HD / 2);
-  for (int c = lane; c < HD; c += 64) {
-    int up;
-    const int byte = which ? value_byte<HD>(at, c, up) : key_byte<HD>(at, c, up);
-    const int pair = which ? c + 16 : c + 2;  // the channel in the upper nibble of the same byte
-    if (!up) out[byte] = code[c] | (code[pair] << 4);
+  const bool none = any || !(span < INFINITY);
+  const bf16_raw sb = none ? 0x7fc0 : span < 0x1p-100f ? 0 : f2bf(span / 15.f), mb = none ? 0x7fc0 : f2bf(lo);
+  scale_min = sb | ((unsigned)mb << 16);
+  const float s = bf2f(sb), r = __builtin_amdgcn_rcpf(s), hs = 0.5f * s;
+  unsigned w = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    // rint(d / s) without a division: s has 8 bits, so d - c s is exact, and it decides the ties and what the approximate quotient got wrong
+    const float d = v[i] - lo;
+    float c = rintf(d * r);
+    const float e = fmaf(-c, s, d);
+    unsigned k = (unsigned)(int)c;
+    if (e > hs || (e == hs && (k & 1))) k += 1;
+    if (e < -hs || (e == -hs && (k & 1))) k -= 1;
+    w |= min(k, 15u) << (4 * i);
   }
-  if (lane == 0) ((unsigned*)p.scales)[plane * p.page + at] = sb | ((unsigned)mb << 16);
+  return (none || sb == 0) ? 0u : w;
+}
+
+template <int HD>
+__global__ __launch_bounds__(256) void kv4_append_kernel(const grove_kv4_append_params p, const int vec) {
+  constexpr int G = HD / 8, R = 64 / G;
+  const int lane = threadIdx.x & 63, g = lane & (G - 1);
+  const int64_t unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);  // (rows of a wave, head), heads side by side
+  const int head = (int)(unit % p.kv), row = (int)(unit / p.kv) * R + lane / G;
+  if ((unit / p.kv) * R >= p.rows) return;
+  int pg = 0, at = 0;
+  const bool ok = slot_of(p.slots, row, p.rows, p.page, p.pages, pg, at);
+  const int r = ok ? row : 0;
+  u32x4_t x[2];
+  const bf16_raw* kp = (const bf16_raw*)p.k + r * p.sk_row + head * p.sk_head + 8 * g;
+  const bf16_raw* vp = (const bf16_raw*)p.v + r * p.sv_row + head * p.sv_head + 8 * g;
+  if (vec) {
+    x[0] = *(const u32x4_t*)kp;
+    x[1] = *(const u32x4_t*)vp;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      x[0][i] = kp[2 * i] | ((unsigned)kp[2 * i + 1] << 16);
+      x[1][i] = vp[2 * i] | ((unsigned)vp[2 * i + 1] << 16);
+    }
+  }
+  unsigned sm[2];
+  const unsigned wk = quantise<G>(x[0], sm[0]), wv = quantise<G>(x[1], sm[1]);
+  const int64_t plane = (int64_t)pg * 2 * p.kv + head;
+  unsigned char* kc = (unsigned char*)p.codes + plane * p.page * (HD / 2);
+  unsigned char* vc = kc + (int64_t)p.kv * p.page * (HD / 2) + (at >> 2) * (2 * HD);
+  if (ok) {
+    // channels 0, 2, 4, 6 in the low half, 1, 3, 5, 7 in the high half
+    unsigned e = wk & 0x0f0f0f0fu, o = (wk >> 4) & 0x0f0f0f0fu;
+    e = (e | e >> 4) & 0x00ff00ffu;
+    o = (o | o >> 4) & 0x00ff00ffu;
+    const unsigned word = ((e | e >> 8) & 0xffffu) | (o | o >> 8) << 16;
+    *(unsigned*)(kc + at * (HD / 2) + ((g & 3) * (HD / 32) + (g >> 2)) * 4) = word;
+    if (g == 0) {
+      ((unsigned*)p.scales)[plane * p.page + at] = sm[0];
+      ((unsigned*)p.scales)[(plane + p.kv) * p.page + at] = sm[1];
+    }
+  }
+  const int tp = (at >> 1) & 1, par = at & 1;
+  if constexpr (HD == 32) {
+    const unsigned t = __shfl_xor(wv, 2, 64), a = (g & 2) ? t >> 16 : wv, b = (g & 2) ? wv >> 16 : t;  // j = 0 and 1 of this lane's four places
+    if (ok)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) vc[(8 * (g & 1) + 2 * (g & 2) + i) * 4 + par * 2 + tp] = (unsigned char)((a >> (4 * i) & 15) | (b >> (4 * i) & 15) << 4);
+  } else {
+    const unsigned w = byte_transpose(wv, g);
+    const int m = 8 * (g & 1) + (g & 6), jq = g >> 3;
+    bf16_raw* y = (bf16_raw*)(vc + m * (HD / 8) + (jq * 2 + tp) * 4 + par * 2);
+    if (ok) {
+      y[0] = (bf16_raw)low_nibbles(w);
+      y[HD / 16] = (bf16_raw)low_nibbles(w >> 4);
+    }
+  }
 }
 
 template <int HD, typename T>
-__global__ __launch_bounds__(64) void kv4_read_kernel(const grove_kv4_read_params p) {
-  const int lane = threadIdx.x, row = blockIdx.x, head = blockIdx.y, which = blockIdx.z;
+__global__ __launch_bounds__(256) void kv4_read_kernel(const grove_kv4_read_params p) {
+  constexpr int G = HD / 8, R = 64 / G;
+  const int lane = threadIdx.x & 63, g = lane & (G - 1);
+  const int64_t unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int head = (int)(unit % p.kv), row = (int)(unit / p.kv) * R + lane / G;
+  if ((unit / p.kv) * R >= p.rows) return;
   int pg = 0, at = 0;
-  const bool ok = slot_of(p.slots, row, p.page, p.pages, pg, at);
-  const int64_t plane = ((int64_t)pg * 2 + which) * p.kv + head;
-  const unsigned char* in = (const unsigned char*)p.codes + plane * p.page * (HD / 2);
-  T* y = (T*)(which ? p.v : p.k) + ((int64_t)row * p.kv + head) * HD;
-  const unsigned sm = ok ? ((const unsigned*)p.scales)[plane * p.page + at] : 0;
-  for (int c = lane; c < HD; c += 64) {
-    int up;
-    const int byte = which ? value_byte<HD>(at, c, up) : key_byte<HD>(at, c, up);
-    const int code = ok ? (in[byte] >> (4 * up)) & 15 : 0;
-    const float v = fmaf((float)code, bf_lo(sm), bf_hi(sm));
-    if constexpr (sizeof(T) == 4) y[c] = v; else y[c] = f2bf(v);
+  const bool ok = slot_of(p.slots, row, p.rows, p.page, p.pages, pg, at);
+  const int64_t plane = (int64_t)pg * 2 * p.kv + head;
+  const unsigned char* kc = (const unsigned char*)p.codes + plane * p.page * (HD / 2);
+  const unsigned char* vc = kc + (int64_t)p.kv * p.page * (HD / 2) + (at >> 2) * (2 * HD);
+  const unsigned sk = ((const unsigned*)p.scales)[plane * p.page + at], sv = ((const unsigned*)p.scales)[(plane + p.kv) * p.page + at];
+  const unsigned word = *(const unsigned*)(kc + at * (HD / 2) + ((g & 3) * (HD / 32) + (g >> 2)) * 4);
+  const unsigned wk = spread_nibbles(word & 0xffffu) | spread_nibbles(word >> 16) << 4;
+  const int tp = (at >> 1) & 1, par = at & 1;
+  unsigned wv = 0;
+  if constexpr (HD == 32) {
+    unsigned a = 0, b = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const unsigned c = vc[(8 * (g & 1) + 2 * (g & 2) + i) * 4 + par * 2 + tp];
+      a |= (c & 15) << (4 * i);
+      b |= (c >> 4) << (4 * i);
+    }
+    const unsigned give = (g & 2) ? a : b, t = __shfl_xor(give, 2, 64);  // j = 0 goes to the lane with j = 0, j = 1 to the other
+    wv = (g & 2) ? t | b << 16 : a | t << 16;
+  } else {
+    const int m = 8 * (g & 1) + (g & 6), jq = g >> 3;
+    const bf16_raw* y = (const bf16_raw*)(vc + m * (HD / 8) + (jq * 2 + tp) * 4 + par * 2);
+    wv = byte_transpose(spread_nibbles(y[0]) | spread_nibbles(y[HD / 16]) << 4, g);
+  }
+  if (row >= p.rows) return;
+#pragma unroll
+  for (int which = 0; which < 2; ++which) {
+    const unsigned w = which ? wv : wk, sm = which ? sv : sk;
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = ok ? fmaf((float)(w >> (4 * i) & 15), bf_lo(sm), bf_hi(sm)) : 0.f;
+    T* y = (T*)(which ? p.v : p.k) + ((int64_t)row * p.kv + head) * HD + 8 * g;
+    if constexpr (sizeof(T) == 4) {
+      *(f32x4_t*)y = (f32x4_t){v[0], v[1], v[2], v[3]};
+      *(f32x4_t*)(y + 4) = (f32x4_t){v[4], v[5], v[6], v[7]};
+    } else {
+      *(u32x4_t*)y = (u32x4_t){pack2bf(v[0], v[1]), pack2bf(v[2], v[3]), pack2bf(v[4], v[5]), pack2bf(v[6], v[7])};
+    }
   }
 }
 
@@ -553,6 +651,8 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(const grove_kv4_attn_para
     if (HD >= 64 || lane < HD) y[lane + 64 * i] = some ? f2bf(o[i] / L) : (bf16_raw)0;
 }
 
+// blocks of four waves for every (rows of a wave, head)
+int64_t kv4_units(int rows, int kv, int hd) { return (((int64_t)rows + 512 / hd - 1) / (512 / hd) * kv + 3) / 4; }
 bool page_ok(int page) { return page == 16 || page == 32 || page == 64 || page == 128 || page == 256; }
 bool hd_ok(int hd) { return hd == 32 || hd == 64 || hd == 128 || hd == 256; }
 
@@ -575,7 +675,10 @@ extern "C" int grove_kv4_append(const grove_kv4_append_params* p, void* stream) 
   if (p->rows == 0) return GROVE_OK;
   GROVE_CHECK(p->k && p->v && p->codes && p->scales && p->slots, GROVE_E_SHAPE, "kv4_append: null pointer");
   GROVE_CHECK(((uintptr_t)p->codes & 15) == 0 && ((uintptr_t)p->scales & 15) == 0, GROVE_E_ALIGN, "kv4_append: the cache must be 16-byte aligned");
-#define LAUNCH(HD) hipLaunchKernelGGL(kv4_append_kernel<HD>, dim3((unsigned)p->rows, (unsigned)p->kv, 2), dim3(64), 0, (hipStream_t)stream, *p)
+  GROVE_CHECK(kv4_units(p->rows, p->kv, p->hd) <= 0x7fffffff, GROVE_E_SHAPE, "kv4_append: too many rows");
+  const dim3 grid((unsigned)kv4_units(p->rows, p->kv, p->hd));
+  const int vec = (((uintptr_t)p->k | (uintptr_t)p->v) & 15) == 0 && p->sk_row % 8 == 0 && p->sk_head % 8 == 0 && p->sv_row % 8 == 0 && p->sv_head % 8 == 0;
+#define LAUNCH(HD) hipLaunchKernelGGL(kv4_append_kernel<HD>, grid, dim3(256), 0, (hipStream_t)stream, *p, vec)
   KV4_HD(p->hd, LAUNCH)
 #undef LAUNCH
   GROVE_LAUNCH_CHECK();
@@ -587,11 +690,13 @@ extern "C" int grove_kv4_read(const grove_kv4_read_params* p, void* stream) {
   KV4_SHAPE(p, "kv4_read");
   if (p->rows == 0) return GROVE_OK;
   GROVE_CHECK(p->k && p->v && p->codes && p->scales && p->slots, GROVE_E_SHAPE, "kv4_read: null pointer");
-  GROVE_CHECK(((uintptr_t)p->codes & 15) == 0 && ((uintptr_t)p->scales & 15) == 0, GROVE_E_ALIGN, "kv4_read: the cache must be 16-byte aligned");
-  const dim3 grid((unsigned)p->rows, (unsigned)p->kv, 2);
-#define LAUNCH(HD)                                                                                                     \
-  if (p->f32) hipLaunchKernelGGL((kv4_read_kernel<HD, float>), grid, dim3(64), 0, (hipStream_t)stream, *p);            \
-  else hipLaunchKernelGGL((kv4_read_kernel<HD, bf16_raw>), grid, dim3(64), 0, (hipStream_t)stream, *p)
+  GROVE_CHECK((((uintptr_t)p->codes | (uintptr_t)p->scales | (uintptr_t)p->k | (uintptr_t)p->v) & 15) == 0, GROVE_E_ALIGN,
+              "kv4_read: the cache and the outputs must be 16-byte aligned");
+  GROVE_CHECK(kv4_units(p->rows, p->kv, p->hd) <= 0x7fffffff, GROVE_E_SHAPE, "kv4_read: too many rows");
+  const dim3 grid((unsigned)kv4_units(p->rows, p->kv, p->hd));
+#define LAUNCH(HD)                                                                                              \
+  if (p->f32) hipLaunchKernelGGL((kv4_read_kernel<HD, float>), grid, dim3(256), 0, (hipStream_t)stream, *p);    \
+  else hipLaunchKernelGGL((kv4_read_kernel<HD, bf16_raw>), grid, dim3(256), 0, (hipStream_t)stream, *p)
   KV4_HD(p->hd, LAUNCH)
 #undef LAUNCH
   GROVE_LAUNCH_CHECK();

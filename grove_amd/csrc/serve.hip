@@ -16,29 +16,77 @@ __device__ __forceinline__ void turn(int pos, double freq, float& s, float& c) {
   sincospif((float)(2.0 * (t - rint(t))), &s, &c);
 }
 
-// One thread per pair; the channels behind `rot` are copied by the threads behind the pairs.
-template <typename T>
-__global__ __launch_bounds__(256) void rotary_kernel(const grove_rotary_params p) {
-  const int half = p.rot >> 1, per = half + (p.x == p.y ? 0 : p.hd - p.rot);
-  const int64_t n = (int64_t)p.rows * p.heads * per;
-  for (int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x; e < n; e += (int64_t)gridDim.x * 256) {
-    const int i = (int)(e % per);
-    const int64_t rh = e / per;
-    const int h = (int)(rh % p.heads), r = (int)(rh / p.heads);
-    const T* x = (const T*)p.x + r * p.sx_row + h * p.sx_head;
-    T* y = (T*)p.y + r * p.sy_row + h * p.sy_head;
-    if (i >= half) {
-      y[p.rot + i - half] = x[p.rot + i - half];
-      continue;
-    }
+// A block makes cos and sin of its rows once, in LDS (fp64 reduction and sincospif are some 60 instructions a pair, and every head of a row shares
+// them), then streams the heads: each thread takes E channels of a pair's first member and, in the half layout, the E of its second (16 bytes each
+// where everything is aligned; E = 1 pair otherwise). Bound by memory: everything is read once and written once.
+constexpr int ROT_THREADS = 256, ROT_TABLE = 2048;  // pairs that a block's table holds
+
+__device__ __forceinline__ void rot_ld(const float* p, float (&v)[4]) {
+  const f32x4_t x = *(const f32x4_t*)p;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = x[i];
+}
+__device__ __forceinline__ void rot_ld(const bf16_raw* p, float (&v)[8]) {
+  const u32x4_t x = *(const u32x4_t*)p;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) { v[2 * i] = bf_lo(x[i]); v[2 * i + 1] = bf_hi(x[i]); }
+}
+__device__ __forceinline__ void rot_st(float* p, const float (&v)[4]) { *(f32x4_t*)p = (f32x4_t){v[0], v[1], v[2], v[3]}; }
+__device__ __forceinline__ void rot_st(bf16_raw* p, const float (&v)[8]) {
+  *(u32x4_t*)p = (u32x4_t){pack2bf(v[0], v[1]), pack2bf(v[2], v[3]), pack2bf(v[4], v[5]), pack2bf(v[6], v[7])};
+}
+template <typename T> __device__ __forceinline__ void rot_ld(const T* p, float (&v)[1]) { v[0] = ld1(p); }
+template <typename T> __device__ __forceinline__ void rot_st(T* p, const float (&v)[1]) { st1(p, v[0]); }
+
+// rpb rows and hpb heads per block; grid (row groups, head groups).
+template <typename T, int E, bool INTERLEAVED>
+__global__ __launch_bounds__(ROT_THREADS) void rotary_kernel(const grove_rotary_params p, const int rpb, const int hpb) {
+  __shared__ __attribute__((aligned(16))) float s_c[ROT_TABLE], s_s[ROT_TABLE];
+  const int tid = threadIdx.x, half = p.rot >> 1, row0 = blockIdx.x * rpb, nr = min(rpb, p.rows - row0), h0 = blockIdx.y * hpb, nh = min(hpb, p.heads - h0);
+  const float sign = p.backward ? -p.mscale : p.mscale;
+  for (int e = tid; e < nr * half; e += ROT_THREADS) {
+    const int r = e / half, i = e - r * half;
     float s, c;
-    turn(p.pos[r], p.freq[i], s, c);
-    c *= p.mscale;
-    s *= p.backward ? -p.mscale : p.mscale;
-    const int ia = p.interleaved ? 2 * i : i, ib = p.interleaved ? 2 * i + 1 : i + half;
-    const float a = ld1(x + ia), b = ld1(x + ib);
-    st1(y + ia, a * c - b * s);
-    st1(y + ib, b * c + a * s);
+    turn(p.pos[row0 + r], p.freq[i], s, c);
+    s_c[e] = c * p.mscale;
+    s_s[e] = s * sign;
+  }
+  __syncthreads();
+  // items of a (row, head): the rotated ones, then the ones that pass through (nothing to do in place)
+  constexpr int STEP = INTERLEAVED && E == 1 ? 2 : E;  // channels of an item, and of an item's first member in the half layout
+  const int turned = INTERLEAVED ? p.rot / STEP : half / STEP, per = turned + (p.x == p.y ? 0 : (p.hd - p.rot) / E), n = nr * nh * per;
+  for (int e = tid; e < n; e += ROT_THREADS) {
+    const int rh = e / per, i = e - rh * per, r = rh / nh, h = h0 + rh - r * nh;
+    const T* x = (const T*)p.x + (row0 + r) * p.sx_row + h * p.sx_head;
+    T* y = (T*)p.y + (row0 + r) * p.sy_row + h * p.sy_head;
+    float a[E], b[E];
+    if (i >= turned) {
+      const int c = p.rot + (i - turned) * E;
+      rot_ld(x + c, a);
+      rot_st(y + c, a);
+    } else if constexpr (INTERLEAVED && E > 1) {
+      rot_ld(x + i * E, a);
+      const int t = r * half + i * (E / 2);
+#pragma unroll
+      for (int k = 0; k < E; k += 2) {
+        const float c = s_c[t + k / 2], s = s_s[t + k / 2];
+        b[k] = a[k] * c - a[k + 1] * s;
+        b[k + 1] = a[k + 1] * c + a[k] * s;
+      }
+      rot_st(y + i * E, b);
+    } else {
+      const int ia = INTERLEAVED ? 2 * i : i * E, ib = INTERLEAVED ? 2 * i + 1 : i * E + half, t = r * half + i * E;
+      rot_ld(x + ia, a);
+      rot_ld(x + ib, b);
+#pragma unroll
+      for (int k = 0; k < E; ++k) {
+        const float c = s_c[t + k], s = s_s[t + k], u = a[k] * c - b[k] * s;
+        b[k] = b[k] * c + a[k] * s;
+        a[k] = u;
+      }
+      rot_st(y + ia, a);
+      rot_st(y + ib, b);
+    }
   }
 }
 
@@ -245,14 +293,31 @@ __global__ __launch_bounds__(VD_THREADS) void verify_drafts_kernel(const grove_v
 }  // namespace
 
 extern "C" int grove_rotary(const grove_rotary_params* p, void* stream) {
-  GROVE_CHECK(p && p->rows >= 0 && p->heads >= 0 && p->hd > 0 && p->rot >= 0 && p->rot <= p->hd && (p->rot & 1) == 0, GROVE_E_SHAPE, "rotary: bad shape");
+  GROVE_CHECK(p && p->rows >= 0 && p->heads >= 0 && p->hd > 0 && p->rot >= 0 && p->rot <= p->hd && (p->rot & 1) == 0 && (int64_t)p->heads * p->hd < (1 << 28),
+              GROVE_E_SHAPE, "rotary: bad shape");
   if (p->rows == 0 || p->heads == 0) return GROVE_OK;
   GROVE_CHECK(p->x && p->y && p->pos && (p->freq || p->rot == 0), GROVE_E_SHAPE, "rotary: null pointer");
   GROVE_CHECK(p->x != p->y || (p->sx_row == p->sy_row && p->sx_head == p->sy_head), GROVE_E_SHAPE, "rotary: in place needs equal strides");
-  const int64_t n = (int64_t)p->rows * p->heads * p->hd;
-  const unsigned blocks = (unsigned)((n + 255) / 256 > 65536 ? 65536 : (n + 255) / 256);
-  if (p->f32) hipLaunchKernelGGL(rotary_kernel<float>, dim3(blocks), dim3(256), 0, (hipStream_t)stream, *p);
-  else hipLaunchKernelGGL(rotary_kernel<bf16_raw>, dim3(blocks), dim3(256), 0, (hipStream_t)stream, *p);
+  // 16 bytes at a time where every piece of a (row, head) starts at a multiple of 16 bytes: the pairs' second members and what passes through too
+  const int es = p->f32 ? 4 : 2, E = 16 / es;
+  auto whole = [&](int64_t v) { return v % E == 0; };
+  const bool vec = (((uintptr_t)p->x | (uintptr_t)p->y) & 15) == 0 && whole(p->sx_row) && whole(p->sx_head) && whole(p->sy_row) && whole(p->sy_head) &&
+                   whole(p->interleaved ? p->rot : p->rot / 2) && whole(p->hd - p->rot);
+  const int half = p->rot / 2;
+  GROVE_CHECK(half <= ROT_TABLE, GROVE_E_SHAPE, "rotary: at most %d rotated channels", 2 * ROT_TABLE);
+  // A block per row and half a dozen heads while there are few rows (their latency counts), rows whole once they fill the chip, and several rows a
+  // block while its items would not keep 256 threads busy.
+  const int items = p->hd / (vec ? E : 1);
+  int rpb = 1, hpb = p->heads;
+  while (hpb > 1 && (int64_t)p->rows * ((p->heads + hpb - 1) / hpb) < 512 && hpb * items > 2 * ROT_THREADS) hpb = (hpb + 1) / 2;
+  while (hpb == p->heads && 2 * rpb * (half ? half : 1) <= ROT_TABLE && rpb * p->heads * items < 8 * ROT_THREADS && p->rows / rpb > 2048) rpb *= 2;
+  const dim3 grid((unsigned)((p->rows + rpb - 1) / rpb), (unsigned)((p->heads + hpb - 1) / hpb));
+#define LAUNCH(T, E, I) hipLaunchKernelGGL((rotary_kernel<T, E, I>), grid, dim3(ROT_THREADS), 0, (hipStream_t)stream, *p, rpb, hpb)
+#define LAUNCH2(T, E) do { if (p->interleaved) LAUNCH(T, E, true); else LAUNCH(T, E, false); } while (0)
+  if (p->f32) { if (vec) LAUNCH2(float, 4); else LAUNCH2(float, 1); }
+  else { if (vec) LAUNCH2(bf16_raw, 8); else LAUNCH2(bf16_raw, 1); }
+#undef LAUNCH2
+#undef LAUNCH
   GROVE_LAUNCH_CHECK();
   return GROVE_OK;
 }
