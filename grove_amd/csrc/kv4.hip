@@ -18,10 +18,12 @@ __device__ __forceinline__ bool slot_of(const int* slots, int row, int rows, int
 // memory for many rows, by the chain slot -> row -> page for few.
 
 // lane g's word holds the nibbles of channels 8 g + 0..7 (g = 2 j + half of the 16 places): a 4 x 4 transpose of bytes over the lanes j = 4 jq + 0..3
+template <int CTRL> __device__ __forceinline__ int lanes(int v) { return __builtin_amdgcn_update_dpp(0, v, CTRL, 0xf, 0xf, true); }
+constexpr int XOR1 = 0xB1, XOR2 = 0x4E, XOR3 = 0x1B, XOR7 = 0x141, XOR15 = 0x140;  // data-parallel moves within 16 lanes: no trip through LDS
 __device__ __forceinline__ unsigned byte_transpose(unsigned w, int g) {
-  unsigned t = __shfl_xor(w, 2, 64);
+  unsigned t = lanes<XOR2>(w);
   w = (g & 2) ? __builtin_amdgcn_perm(t, w, 0x03070105) : __builtin_amdgcn_perm(t, w, 0x06020400);
-  t = __shfl_xor(w, 4, 64);
+  t = lanes<XOR3>(lanes<XOR7>(w));
   return (g & 4) ? __builtin_amdgcn_perm(t, w, 0x03020706) : __builtin_amdgcn_perm(t, w, 0x05040100);
 }
 __device__ __forceinline__ unsigned low_nibbles(unsigned w) {  // the low nibbles of the four bytes side by side
@@ -35,44 +37,51 @@ __device__ __forceinline__ unsigned spread_nibbles(unsigned w) {  // and back
 }
 
 // The eight codes of a lane, nibble i = channel i; and the row's scale and minimum. G lanes share the row.
+// Minimum and maximum run on the bf16 bits as ordered integers (sign and magnitude -> two's complement), two at a time; infinities and NaN are the
+// values outside +-0x7f7f. Quotients x / y: an approximate one, its exact remainder, one correction: right where x / y has few bits, as the ties of
+// both roundings have (a bf16 of 8 bits times 15, a bf16 times k + 1/2), and off by no more than its last bit elsewhere.
 template <int G>
 __device__ __forceinline__ unsigned quantise(const u32x4_t x, unsigned& scale_min) {
-  float v[8], lo, hi;
-  bool bad = false;
+  typedef __attribute__((ext_vector_type(2))) short s16x2_t;
+  auto ordered = [](unsigned b) {
+    const s16x2_t a = __builtin_bit_cast(s16x2_t, b);
+    return a ^ ((a >> 15) & (s16x2_t){0x7fff, 0x7fff});
+  };
+  s16x2_t lo2 = ordered(x[0]), hi2 = lo2;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    v[2 * i] = bf_lo(x[i]);
-    v[2 * i + 1] = bf_hi(x[i]);
-    bad |= ((x[i] & 0x7f80u) == 0x7f80u) | ((x[i] & 0x7f800000u) == 0x7f800000u);
+  for (int i = 1; i < 4; ++i) {
+    const s16x2_t o = ordered(x[i]);
+    lo2 = __builtin_elementwise_min(lo2, o);
+    hi2 = __builtin_elementwise_max(hi2, o);
   }
-  lo = hi = v[0];
-#pragma unroll
-  for (int i = 1; i < 8; ++i) { lo = fminf(lo, v[i]); hi = fmaxf(hi, v[i]); }
-  int any = bad;
-#pragma unroll
-  for (int o = 1; o < G; o <<= 1) {
-    lo = fminf(lo, __shfl_xor(lo, o, 64));
-    hi = fmaxf(hi, __shfl_xor(hi, o, 64));
-    any |= __shfl_xor(any, o, 64);
-  }
-  const float span = hi - lo;
-  const bool none = any || !(span < INFINITY);
-  const bf16_raw sb = none ? 0x7fc0 : span < 0x1p-100f ? 0 : f2bf(span / 15.f), mb = none ? 0x7fc0 : f2bf(lo);
+  int lo = min((int)lo2[0], (int)lo2[1]), hi = max((int)hi2[0], (int)hi2[1]);
+  lo = min(lo, lanes<XOR1>(lo));
+  hi = max(hi, lanes<XOR1>(hi));
+  lo = min(lo, lanes<XOR2>(lo));
+  hi = max(hi, lanes<XOR2>(hi));
+  if constexpr (G >= 8) { lo = min(lo, lanes<XOR7>(lo)); hi = max(hi, lanes<XOR7>(hi)); }
+  if constexpr (G >= 16) { lo = min(lo, lanes<XOR15>(lo)); hi = max(hi, lanes<XOR15>(hi)); }
+  if constexpr (G >= 32) { lo = min(lo, __shfl_xor(lo, 16, 64)); hi = max(hi, __shfl_xor(hi, 16, 64)); }
+  const unsigned lob = (unsigned)(lo ^ ((lo >> 15) & 0x7fff)) & 0xffffu, hib = (unsigned)(hi ^ ((hi >> 15) & 0x7fff)) & 0xffffu;
+  const float lof = bf_lo(lob), span = bf_lo(hib) - lof;
+  const bool none = hi >= 0x7f80 || lo <= (int)(short)0x807f || !(span < INFINITY);
+  float q15 = span * (1.f / 15.f);
+  q15 = fmaf(fmaf(-q15, 15.f, span), 1.f / 15.f, q15);
+  const bf16_raw sb = none ? 0x7fc0 : span < 0x1p-100f ? 0 : f2bf(q15), mb = none ? 0x7fc0 : (bf16_raw)lob;
   scale_min = sb | ((unsigned)mb << 16);
-  const float s = bf2f(sb), r = __builtin_amdgcn_rcpf(s), hs = 0.5f * s;
+  const float s = bf2f(sb), r = __builtin_amdgcn_rcpf(s);
   unsigned w = 0;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    // rint(d / s) without a division: s has 8 bits, so d - c s is exact, and it decides the ties and what the approximate quotient got wrong
-    const float d = v[i] - lo;
-    float c = rintf(d * r);
-    const float e = fmaf(-c, s, d);
-    unsigned k = (unsigned)(int)c;
-    if (e > hs || (e == hs && (k & 1))) k += 1;
-    if (e < -hs || (e == -hs && (k & 1))) k -= 1;
-    w |= min(k, 15u) << (4 * i);
+    const float d = ((i & 1) ? bf_hi(x[i >> 1]) : bf_lo(x[i >> 1])) - lof;
+    float q = d * r;
+    q = fmaf(fmaf(-q, s, d), r, q);
+    w += __float_as_uint(fminf(q, 15.f) + 0x1p23f) << (4 * i);  // rounded to an integer in the last bits of 2^23 + c
   }
-  return (none || sb == 0) ? 0u : w;
+  unsigned off = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) off += 0x4b000000u << (4 * i);
+  return (none || sb == 0) ? 0u : w - off;
 }
 
 template <int HD>
@@ -117,7 +126,7 @@ __global__ __launch_bounds__(256) void kv4_append_kernel(const grove_kv4_append_
   }
   const int tp = (at >> 1) & 1, par = at & 1;
   if constexpr (HD == 32) {
-    const unsigned t = __shfl_xor(wv, 2, 64), a = (g & 2) ? t >> 16 : wv, b = (g & 2) ? wv >> 16 : t;  // j = 0 and 1 of this lane's four places
+    const unsigned t = lanes<XOR2>(wv), a = (g & 2) ? t >> 16 : wv, b = (g & 2) ? wv >> 16 : t;  // j = 0 and 1 of this lane's four places
     if (ok)
 #pragma unroll
       for (int i = 0; i < 4; ++i) vc[(8 * (g & 1) + 2 * (g & 2) + i) * 4 + par * 2 + tp] = (unsigned char)((a >> (4 * i) & 15) | (b >> (4 * i) & 15) << 4);
@@ -157,7 +166,7 @@ __global__ __launch_bounds__(256) void kv4_read_kernel(const grove_kv4_read_para
       a |= (c & 15) << (4 * i);
       b |= (c >> 4) << (4 * i);
     }
-    const unsigned give = (g & 2) ? a : b, t = __shfl_xor(give, 2, 64);  // j = 0 goes to the lane with j = 0, j = 1 to the other
+    const unsigned give = (g & 2) ? a : b, t = lanes<XOR2>(give);  // j = 0 goes to the lane with j = 0, j = 1 to the other
     wv = (g & 2) ? t | b << 16 : a | t << 16;
   } else {
     const int m = 8 * (g & 1) + (g & 6), jq = g >> 3;
