@@ -195,7 +195,7 @@ class Kv4AttnParams(C.Structure):
 
 
 class VerifyDraftsParams(C.Structure):
-    _fields_ = [("draft", c_vp), ("q", c_vp), ("p", c_vp), ("u", c_vp), ("pick", c_vp), ("count", c_vp), ("tokens", c_vp), ("accepted", c_vp),
+    _fields_ = [("draft", c_vp), ("q", c_vp), ("p", c_vp), ("u", c_vp), ("pick", c_vp), ("count", c_vp), ("tokens", c_vp), ("accepted", c_vp), ("partial", c_vp),
                 ("sq_req", c_i64), ("sq_row", c_i64), ("sp_req", c_i64), ("sp_row", c_i64),
                 ("requests", c_i32), ("drafts", c_i32), ("vocab", c_i32), ("bf16", c_i32)]
 

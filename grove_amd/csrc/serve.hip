@@ -185,9 +185,9 @@ __global__ __launch_bounds__(PT_THREADS) void page_tables_kernel(const grove_pag
 }
 
 // ---------------------------------------------------------------- verification of drafted tokens
-constexpr int VD_THREADS = 1024, VD_WAVES = VD_THREADS / 64;
+constexpr int VD_THREADS = 256, VD_WAVES = VD_THREADS / 64;
 
-// Inclusive sum over the block in fp64; `total` = the block's. Two barriers.
+// Inclusive sum over the block in fp64; `total`: of all. Two barriers.
 __device__ __forceinline__ double block_scan(double v, double* wsum, double& total) {
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
 #pragma unroll
@@ -207,87 +207,218 @@ __device__ __forceinline__ double block_scan(double v, double* wsum, double& tot
   return before + v;
 }
 
-// One block per request: the drafts are tested side by side, then the row where they end is summed by chunks (at most 1024), the chunk
-// that holds the threshold is found by a scan over the chunk sums and searched element by element.
-template <typename T>
-__global__ __launch_bounds__(VD_THREADS) void verify_drafts_kernel(const grove_verify_drafts_params p) {
-  __shared__ double sums[VD_THREADS], wsum[VD_WAVES];
-  __shared__ int s_a, s_min, s_max;
-  __shared__ double s_carry;
-  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, b = blockIdx.x, V = p.vocab;
-  const int n = p.count ? max(0, min(p.count[b], p.drafts)) : p.drafts;
-  const T* P = (const T*)p.p + b * p.sp_req;
-  const T* Q = p.q ? (const T*)p.q + b * p.sq_req : nullptr;
-  const int* draft = p.draft + (int64_t)b * p.drafts;
-  if (tid == 0) s_a = n;
-  __syncthreads();
-  for (int i = tid; i < n; i += VD_THREADS) {
-    const int x = draft[i];
-    bool ok = x >= 0 && x < V;
-    if (ok) {
-      const double q = Q ? (double)ld1(Q + i * p.sq_row + x) : 1.0;
-      ok = (double)p.u[(int64_t)b * p.drafts + i] * q < (double)ld1(P + i * p.sp_row + x);
-    }
-    if (!ok) atomicMin(&s_a, i);
-  }
-  __syncthreads();
-  const int a = s_a;
-  P += a * p.sp_row;
-  if (Q) Q += a * p.sq_row;
-  const int sure = a < n && !Q ? draft[a] : -1;  // a certain drafter's refused token: its mass is what is taken off
-  const int per = (V + VD_THREADS * 1024 - 1) / (VD_THREADS * 1024), chunk = 1024 * per, nchunk = (V + chunk - 1) / chunk;
-  int token = -1;
-  for (int mode = a < n ? 0 : 1; mode < 2; ++mode) {  // 0: what the drafter left over, 1: the target itself
-    auto rest = [&](int j) -> double {
-      double r = (double)ld1(P + j);
-      if (mode == 0) {
-        if (Q) r -= (double)ld1(Q + j);
-        else if (j == sure) r -= 1.0;
-      }
-      return r > 0 ? r : 0.0;
-    };
-    for (int c = w; c < nchunk; c += VD_WAVES) {
-      double s = 0;
-      for (int j = c * chunk + lane; j < min(V, (c + 1) * chunk); j += 64) s += rest(j);
+// Four consecutive values; `vec`: the row starts at a multiple of four values' bytes.
+__device__ __forceinline__ void ld4(const float* p, bool vec, float (&v)[4]) {
+  if (vec) {
+    const f32x4_t x = *(const f32x4_t*)p;
 #pragma unroll
-      for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
-      if (lane == 0) sums[c] = s;
-    }
-    if (tid == 0) { s_min = V; s_max = -1; }
-    __syncthreads();
-    const double own = tid < nchunk ? sums[tid] : 0.0;
-    double total;
-    const double inc = block_scan(own, wsum, total);
-    if (!(total > 0)) { __syncthreads(); continue; }
-    const double thr = (double)p.pick[b] * total;
-    if (tid < nchunk && own > 0) {
-      if (inc > thr) atomicMin(&s_min, tid);
-      atomicMax(&s_max, tid);
-    }
-    __syncthreads();
-    const int c = s_min < V ? s_min : s_max;
-    if (tid == c) s_carry = inc - own;
-    __syncthreads();
-    double carry = s_carry;
-    if (tid == 0) { s_min = V; s_max = -1; }
-    __syncthreads();
-    for (int j0 = c * chunk; j0 < min(V, (c + 1) * chunk); j0 += VD_THREADS) {
-      const int j = j0 + tid;
-      const double r = j < V ? rest(j) : 0.0;
-      double sub;
-      const double cdf = carry + block_scan(r, wsum, sub);
-      if (r > 0) {
-        if (cdf > thr) atomicMin(&s_min, j);
-        atomicMax(&s_max, j);
+    for (int i = 0; i < 4; ++i) v[i] = x[i];
+  } else
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = p[i];
+}
+__device__ __forceinline__ void ld4(const bf16_raw* p, bool vec, float (&v)[4]) {
+  if (vec) {
+    const u32x2_t x = *(const u32x2_t*)p;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) { v[2 * i] = bf_lo(x[i]); v[2 * i + 1] = bf_hi(x[i]); }
+  } else
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = bf2f(p[i]);
+}
+
+__device__ __forceinline__ int drafts_of(const grove_verify_drafts_params& p, int b) { return p.count ? max(0, min(p.count[b], p.drafts)) : p.drafts; }
+
+// The first refused draft of request b (n: none), for all threads of the block; s_a in LDS. One wave tests 64 drafts side by side.
+template <typename T>
+__device__ __forceinline__ int accept(const grove_verify_drafts_params& p, int b, int n, int* s_a) {
+  if (threadIdx.x < 64) {
+    const T* P = (const T*)p.p + b * p.sp_req;
+    const T* Q = p.q ? (const T*)p.q + b * p.sq_req : nullptr;
+    int a = n;
+    for (int i0 = 0; i0 < n && a == n; i0 += 64) {
+      const int i = i0 + threadIdx.x;
+      bool refused = false;
+      if (i < n) {
+        const int x = p.draft[(int64_t)b * p.drafts + i];
+        const float u = p.u[(int64_t)b * p.drafts + i];
+        refused = x < 0 || x >= p.vocab;
+        if (!refused) {
+          const double q = Q ? (double)ld1(Q + i * p.sq_row + x) : 1.0;
+          refused = !((double)u * q < (double)ld1(P + i * p.sp_row + x));
+        }
       }
-      carry += sub;
+      const unsigned long long any = __ballot(refused);
+      if (any) a = i0 + __builtin_ctzll(any);
     }
-    __syncthreads();
-    token = s_min < V ? s_min : s_max;
-    break;
+    if (threadIdx.x == 0) *s_a = a;
   }
+  __syncthreads();
+  return *s_a;
+}
+
+// What request b's last token is drawn from: r = max(p - q, 0) of the refused draft's row, or p itself (plain).
+template <typename T>
+struct rest_row {
+  const T *P, *Q;
+  int sure;  // a certain drafter's refused token: its mass is what is taken off
+  bool vp, vq;
+  __device__ rest_row(const grove_verify_drafts_params& p, int b, int a, bool plain) {
+    P = (const T*)p.p + b * p.sp_req + a * p.sp_row;
+    Q = !plain && p.q ? (const T*)p.q + b * p.sq_req + a * p.sq_row : nullptr;
+    sure = !plain && !p.q ? p.draft[(int64_t)b * p.drafts + a] : -1;
+    vp = ((uintptr_t)P & (4 * sizeof(T) - 1)) == 0;
+    vq = ((uintptr_t)Q & (4 * sizeof(T) - 1)) == 0;
+  }
+  __device__ double one(int j) const {
+    double r = (double)ld1(P + j);
+    if (Q) r -= (double)ld1(Q + j);
+    else if (j == sure) r -= 1.0;
+    return r > 0 ? r : 0.0;
+  }
+  // the sum of [j0, j1), by a wave
+  __device__ double sum(int j0, int j1) const {
+    double s = 0;
+    for (int base = j0; base < j1; base += 1024) {
+      const int lane = threadIdx.x & 63;
+      if (base + 1024 <= j1) {
+        float x[4][4], y[4][4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int j = base + 256 * k + 4 * lane;
+          ld4(P + j, vp, x[k]);
+          if (Q) ld4(Q + j, vq, y[k]);
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            double r = (double)x[k][i];
+            if (Q) r -= (double)y[k][i];
+            else if (base + 256 * k + 4 * lane + i == sure) r -= 1.0;
+            s += r > 0 ? r : 0.0;
+          }
+      } else
+        for (int j = base + lane; j < j1; j += 64) s += one(j);
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
+    return s;
+  }
+};
+__host__ __device__ inline int vd_chunk(int V) { return 1024 * ((V + (1 << 20) - 1) >> 20); }  // at most 1024 chunks
+__host__ __device__ inline int vd_chunks(int V) { return (V + vd_chunk(V) - 1) / vd_chunk(V); }
+
+// The token at `pick` of a row whose chunk sums are in LDS: the chunk by a scan over the sums, then element by element. -1: the row holds nothing.
+struct draw_lds {
+  double sums[1024], wsum[VD_WAVES], before;
+  int low[VD_WAVES], last[VD_WAVES];
+};
+// Of 4 x 256 weights, 4 consecutive ones a thread: the first whose running sum (from `carry`) passes thr, else the last that is not 0, else -1; by
+// ballots (atomics on one LDS word take their lanes one after the other). `sum`: of all; s.before, after a barrier: the sum before the one found.
+__device__ int search(const double (&r)[4], double carry, double thr, draw_lds& s, double& sum, bool& passed) {
+  const int tid = threadIdx.x, w = tid >> 6;
+  const double own = (r[0] + r[1]) + (r[2] + r[3]), before = carry + (block_scan(own, s.wsum, sum) - own);
+  int low = 4, last = -1;
+  double c[5];
+  c[0] = before;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) c[i + 1] = c[i] + r[i];
+#pragma unroll
+  for (int i = 3; i >= 0; --i)
+    if (r[i] > 0) {
+      if (last < 0) last = i;
+      if (c[i + 1] > thr) low = i;
+    }
+  const unsigned long long lows = __ballot(low < 4), some = __ballot(last >= 0);
+  const int l0 = lows ? __builtin_ctzll(lows) : 0, l1 = some ? 63 - __builtin_clzll(some) : 0;
+  const int low_i = __shfl(low, l0, 64), last_i = __shfl(last, l1, 64);
+  if ((tid & 63) == 0) {
+    s.low[w] = lows ? (w * 64 + l0) * 4 + low_i : 1024;
+    s.last[w] = some ? (w * 64 + l1) * 4 + last_i : -1;
+  }
+  __syncthreads();
+  int lo = s.low[0], la = s.last[0];
+#pragma unroll
+  for (int i = 1; i < VD_WAVES; ++i) { lo = min(lo, s.low[i]); la = max(la, s.last[i]); }
+  passed = lo < 1024;
+  const int at = passed ? lo : la;
+  if (at >= 0 && tid == at >> 2) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (i == (at & 3)) s.before = c[i];
+  }
+  return at;
+}
+template <typename T>
+__device__ int draw(const rest_row<T>& row, int V, float pick, draw_lds& s) {
+  const int tid = threadIdx.x, chunk = vd_chunk(V), nchunk = vd_chunks(V);
+  __syncthreads();  // the sums are there
+  double r[4], total = 0, part;
+  bool passed;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r[i] = 4 * tid + i < nchunk ? s.sums[4 * tid + i] : 0.0;
+  block_scan((r[0] + r[1]) + (r[2] + r[3]), s.wsum, total);
+  if (!(total > 0)) return -1;
+  const double thr = (double)pick * total;
+  const int c = search(r, 0.0, thr, s, part, passed);
+  __syncthreads();
+  double carry = s.before;
+  int last = -1;
+  for (int j0 = c * chunk; j0 < min(V, (c + 1) * chunk); j0 += 1024) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r[i] = j0 + 4 * tid + i < V ? row.one(j0 + 4 * tid + i) : 0.0;
+    const int at = search(r, carry, thr, s, part, passed);
+    if (at >= 0) last = j0 + at;
+    if (passed) return last;
+    carry += part;
+    __syncthreads();
+  }
+  return last;
+}
+
+// One block per request. SUMMED: the chunk sums and the number of accepted drafts come from verify_sums_kernel. Otherwise the block forms them; and in
+// either case those of the target alone where the difference leaves nothing.
+template <typename T, bool SUMMED>
+__global__ __launch_bounds__(VD_THREADS) void verify_drafts_kernel(const grove_verify_drafts_params p) {
+  __shared__ draw_lds s;
+  __shared__ int s_a;
+  const int tid = threadIdx.x, b = blockIdx.x, V = p.vocab, n = drafts_of(p, b), nchunk = vd_chunks(V), chunk = vd_chunk(V);
+  const int a = SUMMED ? p.accepted[b] : accept<T>(p, b, n, &s_a);
+  bool ready = SUMMED;
+  if (SUMMED)
+    for (int c = tid; c < nchunk; c += VD_THREADS) s.sums[c] = p.partial[(int64_t)b * nchunk + c];
+  int token = -1;
+  for (int plain = a < n ? 0 : 1; plain < 2 && token < 0; ++plain) {
+    const rest_row<T> row(p, b, a, plain);
+    if (!ready) {
+      __syncthreads();
+      for (int c = tid >> 6; c < nchunk; c += VD_WAVES) {
+        const double sum = row.sum(c * chunk, min(V, (c + 1) * chunk));
+        if ((tid & 63) == 0) s.sums[c] = sum;
+      }
+    }
+    ready = false;
+    token = draw(row, V, p.pick[b], s);
+  }
+  const int* draft = p.draft + (int64_t)b * p.drafts;
   for (int i = tid; i <= p.drafts; i += VD_THREADS) p.tokens[(int64_t)b * (p.drafts + 1) + i] = i < a ? draft[i] : i == a ? token : -1;
-  if (tid == 0) p.accepted[b] = a;
+  if (!SUMMED && tid == 0) p.accepted[b] = a;
+}
+
+// A few blocks per request form the chunk sums (a CU reads some 22 GB/s, so one block takes 12 us over a vocabulary of 32008): each tests the drafts for
+// itself, then a wave takes a chunk at a time.
+template <typename T>
+__global__ __launch_bounds__(256) void verify_sums_kernel(const grove_verify_drafts_params p, const int per) {
+  __shared__ int s_a;
+  const int b = blockIdx.y, V = p.vocab, n = drafts_of(p, b), nchunk = vd_chunks(V), chunk = vd_chunk(V);
+  const int a = accept<T>(p, b, n, &s_a);
+  const rest_row<T> row(p, b, a, a == n);
+  for (int c = blockIdx.x * per + (threadIdx.x >> 6); c < min(nchunk, ((int)blockIdx.x + 1) * per); c += 4) {
+    const double sum = row.sum(c * chunk, min(V, (c + 1) * chunk));
+    if ((threadIdx.x & 63) == 0) p.partial[(int64_t)b * nchunk + c] = sum;
+  }
+  if (blockIdx.x == 0 && threadIdx.x == 0) p.accepted[b] = a;
 }
 
 }  // namespace
@@ -340,8 +471,23 @@ extern "C" int grove_verify_drafts(const grove_verify_drafts_params* p, void* st
   GROVE_CHECK(p && p->requests >= 0 && p->drafts >= 0 && p->vocab > 0 && p->vocab <= (1 << 30), GROVE_E_SHAPE, "verify_drafts: bad shape");
   if (p->requests == 0) return GROVE_OK;
   GROVE_CHECK(p->p && p->pick && p->tokens && p->accepted && ((p->draft && p->u) || p->drafts == 0), GROVE_E_SHAPE, "verify_drafts: null pointer");
-  if (p->bf16) hipLaunchKernelGGL(verify_drafts_kernel<bf16_raw>, dim3((unsigned)p->requests), dim3(VD_THREADS), 0, (hipStream_t)stream, *p);
-  else hipLaunchKernelGGL(verify_drafts_kernel<float>, dim3((unsigned)p->requests), dim3(VD_THREADS), 0, (hipStream_t)stream, *p);
+  const dim3 grid((unsigned)p->requests);
+  if (p->partial) {
+    // a chunk for each wave of a block, several once that makes more than 2048 blocks
+    GROVE_CHECK(p->requests <= 65535, GROVE_E_SHAPE, "verify_drafts: at most 65535 requests with a workspace");
+    const int nchunk = vd_chunks(p->vocab);
+    const int64_t want = ((int64_t)nchunk * p->requests + 2047) / 2048;
+    const int per = want <= 4 ? 4 : (int)(want + 3) / 4 * 4;
+    const dim3 parts((unsigned)((nchunk + per - 1) / per), (unsigned)p->requests);
+    if (p->bf16) hipLaunchKernelGGL(verify_sums_kernel<bf16_raw>, parts, dim3(256), 0, (hipStream_t)stream, *p, per);
+    else hipLaunchKernelGGL(verify_sums_kernel<float>, parts, dim3(256), 0, (hipStream_t)stream, *p, per);
+    GROVE_LAUNCH_CHECK();
+    if (p->bf16) hipLaunchKernelGGL((verify_drafts_kernel<bf16_raw, true>), grid, dim3(VD_THREADS), 0, (hipStream_t)stream, *p);
+    else hipLaunchKernelGGL((verify_drafts_kernel<float, true>), grid, dim3(VD_THREADS), 0, (hipStream_t)stream, *p);
+  } else {
+    if (p->bf16) hipLaunchKernelGGL((verify_drafts_kernel<bf16_raw, false>), grid, dim3(VD_THREADS), 0, (hipStream_t)stream, *p);
+    else hipLaunchKernelGGL((verify_drafts_kernel<float, false>), grid, dim3(VD_THREADS), 0, (hipStream_t)stream, *p);
+  }
   GROVE_LAUNCH_CHECK();
   return GROVE_OK;
 }

@@ -1489,6 +1489,9 @@ def kv4_attn(q, cache, table, kv_len, cu_q, max_q, alpha, *, max_len=None, out=N
     return out
 
 
+_VERIFY_SPLIT = 8192  # vocabulary from which several blocks form a request's sums
+
+
 def verify_drafts(draft, q, p, u, pick, count=None):
     """(tokens int32 [requests, drafts + 1], accepted int32 [requests]): the drafts that the rejection rule accepts and the token after them, -1
     behind (grove_verify_drafts). draft int32 [requests, drafts]; q f32 or bf16 [requests, drafts, vocab] the drafter's probabilities, None for a
@@ -1516,7 +1519,8 @@ def verify_drafts(draft, q, p, u, pick, count=None):
     _need_device(what, p)
     tokens = torch.empty((B, K + 1), dtype=torch.int32, device=p.device)
     accepted = torch.empty(B, dtype=torch.int32, device=p.device)
+    partial = torch.empty(B * min(1024, -(-V // 1024)), dtype=torch.float64, device=p.device) if V > _VERIFY_SPLIT and 0 < B < 512 else None
     a = _lib.VerifyDraftsParams(draft.data_ptr(), qp, p.data_ptr(), u.data_ptr(), pick.data_ptr(), 0 if count is None else count.data_ptr(), tokens.data_ptr(),
-                                accepted.data_ptr(), qb, qr, p.stride(0), p.stride(1), B, K, V, dt == bf16)
+                                accepted.data_ptr(), 0 if partial is None else partial.data_ptr(), qb, qr, p.stride(0), p.stride(1), B, K, V, dt == bf16)
     _launch(what, a, p, draft, q if qp else None, u, pick, count)
     return tokens, accepted

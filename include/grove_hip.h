@@ -745,6 +745,7 @@ typedef struct grove_verify_drafts_params {
   const int32_t* count; /* [requests] or NULL */
   int32_t* tokens;      /* [requests, drafts + 1] out */
   int32_t* accepted;    /* [requests] out */
+  double* partial;      /* NULL: one block per request; or f64 [requests, min(1024, ceil(vocab / 1024))]: several, and a second launch */
   int64_t sq_req, sq_row, sp_req, sp_row;
   int32_t requests, drafts, vocab, bf16;
 } grove_verify_drafts_params;

@@ -557,7 +557,8 @@ def check_verify(dev, d, q, p, u, pick, count=None):
 
 
 @pytest.mark.parametrize("dtype", [f32, bf16])
-@pytest.mark.parametrize("B,K,V", [(1, 1, 1), (3, 2, 5), (40, 4, 320), (8, 4, 32008), (5, 7, 1023), (6, 1, 1025), (2, 3, 128001), (300, 3, 64), (1, 70, 40)])
+@pytest.mark.parametrize("B,K,V", [(1, 1, 1), (3, 2, 5), (40, 4, 320), (8, 4, 32008), (5, 7, 1023), (6, 1, 1025), (2, 3, 128001), (300, 3, 64), (1, 70, 40),
+                                   (2, 1, 1100003), (600, 1, 9001)])
 def test_verify(dev, dtype, B, K, V):
     d, q, p, u, pick = drafts(B, K, V, B + V, dtype)
     check_verify(dev, d, q, p, u, pick)
