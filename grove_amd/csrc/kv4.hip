@@ -615,25 +615,31 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(const grove_kv4_attn_para
   const int64_t unit = WAVES == 1 ? (int64_t)blockIdx.x * 4 + w : (int64_t)blockIdx.x;
   if (unit >= (int64_t)p.rows * p.heads) return;
   const int row = (int)(unit / p.heads), head = (int)(unit - (int64_t)row * p.heads);
-  const bool mine = row >= p.cu_q[0] && row < p.cu_q[p.requests];
+  // (everything is asked for at once: the partial results are there to read whether or not the row is a request's)
+  const float* ml = p.partial + (int64_t)p.rows * p.heads * S * HD + unit * S * 2;
+  const float* part = p.partial + unit * S * HD + min(lane, HD - 1);
+  const int r0 = p.cu_q[0], r1 = p.cu_q[p.requests];
+  const float m_in = ml[2 * min(lane, S - 1)], l_in = ml[2 * min(lane, S - 1) + 1];
+  float x[8][NC];
+  auto ask = [&](int s0) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+#pragma unroll
+      for (int i = 0; i < NC; ++i) x[k][i] = part[(int64_t)min(s0 + k * WAVES, S - 1) * HD + 64 * i];
+  };
+  int s0 = WAVES == 1 ? 0 : w;
+  ask(s0);
+  const bool mine = row >= r0 && row < r1;
   if (!mine && !p.fresh) return;
   bf16_raw* y = (bf16_raw*)p.out + row * p.so_row + (int64_t)head * HD;
   float o[NC] = {}, L = 0.f;
   if (mine) {
-    const float* ml = p.partial + (int64_t)p.rows * p.heads * S * HD + unit * S * 2;
-    const float* part = p.partial + unit * S * HD + min(lane, HD - 1);
-    float ms = NEG, ls = 0.f;
-    if (lane < S) { ms = ml[2 * lane]; ls = ml[2 * lane + 1]; }
-    const bool live = ls != 0.f;  // a split without keys wrote no output
-    const float M = wave_max(live ? ms : NEG), f = !live || ms == NEG ? 0.f : __builtin_amdgcn_exp2f(ms - M);
+    const bool live = lane < S && l_in != 0.f;  // a split without keys wrote no output
+    const float ms = live ? m_in : NEG, ls = live ? l_in : 0.f;
+    const float M = wave_max(ms), f = ms == NEG ? 0.f : __builtin_amdgcn_exp2f(ms - M);
     L = wave_sum(live ? f * ls : 0.f);
     const unsigned long long alive = __ballot(live);
-    for (int s0 = WAVES == 1 ? 0 : w; s0 < S; s0 += 8 * WAVES) {
-      float x[8][NC];
-#pragma unroll
-      for (int k = 0; k < 8; ++k)
-#pragma unroll
-        for (int i = 0; i < NC; ++i) x[k][i] = part[(int64_t)min(s0 + k * WAVES, S - 1) * HD + 64 * i];
+    while (true) {
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
         const int s = s0 + k * WAVES;
@@ -642,6 +648,9 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(const grove_kv4_attn_para
 #pragma unroll
           for (int i = 0; i < NC; ++i) o[i] += fs * x[k][i];
       }
+      s0 += 8 * WAVES;
+      if (s0 >= S) break;
+      ask(s0);
     }
   }
   if constexpr (WAVES > 1) {
@@ -732,7 +741,7 @@ extern "C" int grove_kv4_attn(const grove_kv4_attn_params* p, void* stream) {
 #define RUN(HD, CT)                                                                                                                  \
   do {                                                                                                                               \
     constexpr int lds = 4 * kv4_slots(HD, CT) * kv4_bytes(HD);                                                                       \
-    hipFuncSetAttribute((const void*)kv4_attn_kernel<HD, CT>, hipFuncAttributeMaxDynamicSharedMemorySize, lds);                      \
+    if (lds > 64 * 1024) hipFuncSetAttribute((const void*)kv4_attn_kernel<HD, CT>, hipFuncAttributeMaxDynamicSharedMemorySize, lds);                      \
     hipLaunchKernelGGL((kv4_attn_kernel<HD, CT>), grid, dim3(256), lds, (hipStream_t)stream, *p, shift, vec_q, vec_o);               \
   } while (0)
 #define LAUNCH(HD)                       \
