@@ -277,13 +277,13 @@ constexpr float NEG = -INFINITY;
 constexpr int KV4_WAVES(int hd, int ct) { return hd * ct <= 128 ? 3 : hd * ct <= 256 ? 2 : 1; }
 
 template <int HD, int CT>
-__global__ __launch_bounds__(256, KV4_WAVES(HD, CT)) void kv4_attn_kernel(const grove_kv4_attn_params p, const int shift, const int vec_q, const int vec_o) {
-  constexpr int NK = HD / 32, NJ = HD / 16, HC = HD < 128 ? HD : 128;  // HC channels go through LDS at a time
+__global__ __launch_bounds__(256, KV4_WAVES(HD, CT)) void kv4_attn_kernel(const grove_kv4_attn_params p, const int shift) {
+  constexpr int NK = HD / 32, NJ = HD / 16, CG = CT < 2 ? CT : 2;  // CG tiles of columns hand their outputs through LDS at a time
   constexpr int S = kv4_slots(HD, CT), BYTES = kv4_bytes(HD), OPS = kv4_ops(HD), PART = kv4_part(HD);
-  static_assert(4 * S * BYTES >= (int)sizeof(float) * 4 * 16 * (HC + 4), "the outputs pass through the rings' memory");
+  static_assert(4 * S * BYTES >= (int)sizeof(float) * 4 * 16 * CG * (HD + 4), "the outputs pass through the rings' memory");
   extern __shared__ __attribute__((aligned(1024))) char smem[];
   __shared__ float s_m[4][16 * CT], s_l[4][16 * CT], s_c[4][16 * CT];
-  float(*s_o)[16][HC + 4] = (float(*)[16][HC + 4])smem;
+  float(*s_o)[16 * CG][HD + 4] = (float(*)[16 * CG][HD + 4])smem;
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), n16 = lane & 15, h = lane >> 4;
   const int G = p.heads / p.kv, chunks = gridDim.y / p.kv, hk = blockIdx.y / chunks, cc = blockIdx.y - hk * chunks, b = blockIdx.z, sp = blockIdx.x;
   typedef const __attribute__((address_space(4))) int* scalar_ints;  // scalar loads: of inputs that nothing writes meanwhile
@@ -314,11 +314,7 @@ __global__ __launch_bounds__(256, KV4_WAVES(HD, CT)) void kv4_attn_kernel(const 
 #pragma unroll
       for (int t = 0; t < NK; ++t) {
         u32x4_t r = {0, 0, 0, 0};
-        if (c < cols) {
-          if (vec_q) r = *(const u32x4_t*)(x + 32 * t);
-          else
-            for (int e = 0; e < 4; ++e) r[e] = x[32 * t + 2 * e] | ((unsigned)x[32 * t + 2 * e + 1] << 16);
-        }
+        if (c < cols) r = *(const u32x4_t*)(x + 32 * t);
         q[ct][t] = __builtin_bit_cast(bf16x8_t, r);
       }
     }
@@ -499,19 +495,19 @@ __global__ __launch_bounds__(256, KV4_WAVES(HD, CT)) void kv4_attn_kernel(const 
     }
     return true;
   };
-  bool fresh_q = true, again;
+  bool first = true, again;
+  ahead = tile0 + w;
+  if (ahead < tile1) ask_pages();
+  ask_q();
   do {
     again = false;
-    tile = ahead = tile0 + w;
+    tile = ahead;
     to = from = 0;
     bad = 0;
-    if (tile < tile1) ask_pages();
-    if (fresh_q) ask_q();
-#pragma unroll
-    for (int i = 0; i < S - 1; ++i)
-      if (ahead < tile1) issue();
-    if (fresh_q) use_q();
-    fresh_q = false;
+#pragma unroll 1
+    for (int i = 0; i < S - 1 && ahead < tile1; ++i) issue();  // (rolled: what a block runs once is fetched cold, and its length counts)
+    if (first) use_q();
+    first = false;
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
       l[ct] = cst[ct] = 0.f;
@@ -531,6 +527,8 @@ __global__ __launch_bounds__(256, KV4_WAVES(HD, CT)) void kv4_attn_kernel(const 
       again = __any(again);
       if (again) {
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the tiles in flight land before their slots are asked for again
+        ahead = tile0 + w;
+        ask_pages();
         break;
       }
     }
@@ -550,57 +548,52 @@ __global__ __launch_bounds__(256, KV4_WAVES(HD, CT)) void kv4_attn_kernel(const 
     }
   }
   __syncthreads();  // (the rings are read, nothing is in flight: their memory takes the outputs)
-  const bool split = p.n_split > 1;
-  const int oc = tid >> 4, och = (tid & 15) * (HC / 16);
+  auto joint = [&](int col) { return fmaxf(fmaxf(s_m[0][col], s_m[1][col]), fmaxf(s_m[2][col], s_m[3][col])); };
+  auto part = [&](float mw, float M) { return mw == NEG ? 0.f : __builtin_amdgcn_exp2f(mw - M); };
+  constexpr int EL = HD / 16;  // 16 threads a column
+  const int och = (tid & 15) * EL;
 #pragma unroll
-  for (int ct = 0; ct < CT; ++ct) {
-    auto joint = [&](int col) { return fmaxf(fmaxf(s_m[0][col], s_m[1][col]), fmaxf(s_m[2][col], s_m[3][col])); };
-    auto part = [&](float mw, float M) { return mw == NEG ? 0.f : __builtin_amdgcn_exp2f(mw - M); };
-    const float f = part(s_m[w][ct * 16 + n16], joint(ct * 16 + n16));
-    const int col = ct * 16 + oc, c = col0 + col, i = c / G;
-    const float M = joint(col);
-    float L = 0.f, C = 0.f;
+  for (int g0 = 0; g0 < CT; g0 += CG) {
+    if (g0) __syncthreads();
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const float fk = part(s_m[k][col], M);
-      L += fk * s_l[k][col];
-      C += fk * s_c[k][col];
+    for (int ct = g0; ct < g0 + CG; ++ct) {
+      const float f = part(s_m[w][ct * 16 + n16], joint(ct * 16 + n16));
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) *(f32x4_t*)&s_o[w][(ct - g0) * 16 + n16][16 * j + 4 * h] = acc[ct][j] * f;
     }
-    const int64_t unit = (int64_t)(t0 + i) * p.heads + hk * G + (c - i * G);
-    if (split && c < cols && (tid & 15) == 0) {
-      float* ml = p.partial + (int64_t)p.rows * p.heads * p.n_split * HD + (unit * p.n_split + sp) * 2;
-      ml[0] = M;
-      ml[1] = L;
-    }
+    __syncthreads();
+#pragma unroll 1
+    for (int oc = tid >> 4; oc < 16 * CG; oc += 16) {
+      const int col = g0 * 16 + oc, c = col0 + col, i = c / G;
+      if (c >= cols) break;
+      const float M = joint(col);
+      float L = 0.f, C = 0.f;
 #pragma unroll
-    for (int c0 = 0; c0 < HD; c0 += HC) {
-#pragma unroll
-      for (int j = 0; j < HC / 16; ++j) *(f32x4_t*)&s_o[w][n16][16 * j + 4 * h] = acc[ct][c0 / 16 + j] * f;
-      __syncthreads();
-      if (c < cols) {
-        float o[HC / 16];
-#pragma unroll
-        for (int e = 0; e < HC / 16; ++e) o[e] = C + ((s_o[0][oc][och + e] + s_o[1][oc][och + e]) + (s_o[2][oc][och + e] + s_o[3][oc][och + e]));
-        if (split) {
-          float* y = p.partial + (unit * p.n_split + sp) * HD + c0 + och;
-#pragma unroll
-          for (int e = 0; e < HC / 16; ++e) y[e] = o[e];
-        } else {
-          bf16_raw* y = (bf16_raw*)p.out + (t0 + i) * p.so_row + (int64_t)(hk * G + c - i * G) * HD + c0 + och;
-          const float r = L > 0.f || L != L ? 1.f / L : 0.f;
-          unsigned pk[HC / 32];
-#pragma unroll
-          for (int e = 0; e < HC / 32; ++e) pk[e] = L > 0.f || L != L ? pack2bf(o[2 * e] * r, o[2 * e + 1] * r) : 0u;
-          if (vec_o) {
-#pragma unroll
-            for (int e = 0; e < HC / 32; ++e) ((unsigned*)y)[e] = pk[e];
-          } else {
-#pragma unroll
-            for (int e = 0; e < HC / 16; ++e) y[e] = (bf16_raw)(pk[e >> 1] >> (16 * (e & 1)));
-          }
-        }
+      for (int k = 0; k < 4; ++k) {
+        const float fk = part(s_m[k][col], M);
+        L += fk * s_l[k][col];
+        C += fk * s_c[k][col];
       }
-      __syncthreads();
+      float o[EL];
+#pragma unroll
+      for (int e = 0; e < EL; ++e) o[e] = C + ((s_o[0][oc][och + e] + s_o[1][oc][och + e]) + (s_o[2][oc][och + e] + s_o[3][oc][och + e]));
+      if (p.n_split > 1) {
+        const int64_t unit = (int64_t)(t0 + i) * p.heads + hk * G + (c - i * G), at = unit * p.n_split + sp;
+        if ((tid & 15) == 0) {
+          float* ml = p.partial + (int64_t)p.rows * p.heads * p.n_split * HD + at * 2;
+          ml[0] = M;
+          ml[1] = L;
+        }
+        float* y = p.partial + at * HD + och;
+#pragma unroll
+        for (int e = 0; e < EL; ++e) y[e] = o[e];
+      } else {
+        unsigned* y = (unsigned*)((bf16_raw*)p.out + (t0 + i) * p.so_row + (int64_t)(hk * G + c - i * G) * HD + och);
+        const bool some = L > 0.f || L != L;
+        const float r = 1.f / L;
+#pragma unroll
+        for (int e = 0; e < EL / 2; ++e) y[e] = some ? pack2bf(o[2 * e] * r, o[2 * e + 1] * r) : 0u;
+      }
     }
   }
 }
@@ -731,7 +724,8 @@ extern "C" int grove_kv4_attn(const grove_kv4_attn_params* p, void* stream) {
   GROVE_CHECK(p->n_split >= 1 && p->n_split <= 64 && (p->n_split == 1 || p->partial), GROVE_E_WORKSPACE, "kv4_attn: 1 to 64 splits, more than one with a workspace");
   GROVE_CHECK((int64_t)p->max_pages * p->page <= 0x7fffffff, GROVE_E_SHAPE, "kv4_attn: the table holds more than 2^31 tokens");
   const int shift = __builtin_ctz((unsigned)p->page);
-  const int vec_q = ((uintptr_t)p->q & 15) == 0 && p->sq_row % 8 == 0 && p->sq_head % 8 == 0, vec_o = ((uintptr_t)p->out & 15) == 0 && p->so_row % 8 == 0;
+  GROVE_CHECK(((uintptr_t)p->q & 15) == 0 && p->sq_row % 8 == 0 && p->sq_head % 8 == 0 && ((uintptr_t)p->out & 3) == 0 && p->so_row % 2 == 0, GROVE_E_ALIGN,
+              "kv4_attn: q must be aligned to 16 bytes and out to 4, their strides too");
   // columns that one pass over a key can serve: as few tiles of 16 as hold them, at most 64 (32 at hd 256, whose outputs fill the registers)
   const int64_t cols = (int64_t)(p->max_q < p->rows ? p->max_q : p->rows) * (p->heads / p->kv);
   const int ct = cols <= 16 ? 1 : cols <= 32 || p->hd == 256 ? 2 : 4;
@@ -742,7 +736,7 @@ extern "C" int grove_kv4_attn(const grove_kv4_attn_params* p, void* stream) {
   do {                                                                                                                               \
     constexpr int lds = 4 * kv4_slots(HD, CT) * kv4_bytes(HD);                                                                       \
     if (lds > 64 * 1024) hipFuncSetAttribute((const void*)kv4_attn_kernel<HD, CT>, hipFuncAttributeMaxDynamicSharedMemorySize, lds);                      \
-    hipLaunchKernelGGL((kv4_attn_kernel<HD, CT>), grid, dim3(256), lds, (hipStream_t)stream, *p, shift, vec_q, vec_o);               \
+    hipLaunchKernelGGL((kv4_attn_kernel<HD, CT>), grid, dim3(256), lds, (hipStream_t)stream, *p, shift);               \
   } while (0)
 #define LAUNCH(HD)                       \
   if (ct == 1) RUN(HD, 1);               \

@@ -1446,8 +1446,8 @@ def _kv4_split(pairs, max_len, cols, hd):
 
 
 def kv4_attn(q, cache, table, kv_len, cu_q, max_q, alpha, *, max_len=None, out=None):
-    """Causal attention of every request's new tokens over its 4-bit pages (grove_kv4_attn). q: bf16 [rows, heads, hd], any row and head strides;
-    table int32 [requests, max_pages]; kv_len int32 [requests] keys including the new tokens; cu_q int32 [requests + 1] (page_tables makes both);
+    """Causal attention of every request's new tokens over its 4-bit pages (grove_kv4_attn). q: bf16 [rows, heads, hd], any row and head strides
+    (read in place where they are multiples of 8 from a 16-byte aligned start); table int32 [requests, max_pages]; kv_len int32 [requests] keys including the new tokens; cu_q int32 [requests + 1] (page_tables makes both);
     max_q: the most new tokens that any request has. max_len: the longest kv_len if the host knows it (default: what the table holds); only the
     split of the work goes by it. Returns bf16 [rows, heads * hd]; rows of no request are zero in a new tensor and stay as they were in `out`."""
     what = "kv4_attn"
@@ -1479,6 +1479,11 @@ def kv4_attn(q, cache, table, kv_len, cu_q, max_q, alpha, *, max_len=None, out=N
         if not all(_apart(out, t) for t in (q, codes, scales, table, kv_len, cu_q)):
             _refuse(what, "out overlaps an input")
         orow = out.stride(0)
+        if orow % 2 or out.data_ptr() % 4:
+            _refuse(what, "out must be aligned to 4 bytes, its row stride even")
+    if (qr % 8 and rows > 1) or qh % 8 or q.data_ptr() % 16:  # (an odd start or stride: its rows are laid out anew)
+        q = q.contiguous()
+        qr, qh = heads * hd, hd
     n_split = _kv4_split(B * kv, most * P if max_len is None else max_len, min(max_q, rows) * (heads // kv), hd)
     # the joined splits' workspace: from the allocator at every call, so that calls on other streams and captured graphs have their own
     partial = torch.empty(rows * heads * n_split * (hd + 2), dtype=torch.float32, device=q.device) if n_split > 1 else None
