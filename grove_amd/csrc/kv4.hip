@@ -205,7 +205,7 @@ __global__ __launch_bounds__(256) void kv4_read_kernel(const grove_kv4_read_para
 constexpr int kv4_part(int hd) { return 64 * (hd / 8); }              // bytes of 16 keys' codes
 constexpr int kv4_bytes(int hd) { return 4 * kv4_part(hd) + 256; }    // of a tile: two parts of keys, two of values, scales
 constexpr int kv4_ops(int hd) { return hd / 32 + 1; }
-constexpr int kv4_slots(int hd, int ct) { return hd == 256 ? (ct == 1 ? 2 : 4) : hd == 128 ? (ct == 1 ? 3 : ct == 2 ? 4 : 6) : 4; }
+constexpr int kv4_slots(int hd, int ct) { return hd == 256 ? (ct == 1 ? 2 : 4) : hd == 128 ? (ct == 2 ? 4 : 3) : 4; }
 
 template <int HD>
 struct kv4_tile {
@@ -274,13 +274,19 @@ __device__ __forceinline__ bf16x8_t frag(unsigned a, unsigned b, unsigned c, uns
 
 constexpr float NEG = -INFINITY;
 
-constexpr int KV4_WAVES(int hd, int ct) { return hd * ct <= 128 ? 3 : hd * ct <= 256 ? 2 : 1; }
+constexpr int kv4_waves(int hd, int ct) { return hd * ct <= 128 ? 3 : hd == 256 && ct == 2 ? 1 : 2; }  // a SIMD's, which their registers have to leave room for
+// With 64 columns of 128 the queries stay in LDS, in the operand's order, and are read per tile: in registers they cost the second wave of a SIMD
+// (64 requests x 5 tokens x 8 heads a group over 2048 keys: 85 us, in LDS 67). At 256 x 32 a single wave with its queries in registers and twice the
+// ring is the faster one (72 us against 84).
+constexpr bool kv4_q_lds(int hd, int ct) { return hd == 128 && ct == 4; }
+constexpr int kv4_lds(int hd, int ct) { return 4 * kv4_slots(hd, ct) * kv4_bytes(hd) + (kv4_q_lds(hd, ct) ? 32 * hd * ct + 64 * ct : 0); }
 
 template <int HD, int CT>
-__global__ __launch_bounds__(256, KV4_WAVES(HD, CT)) void kv4_attn_kernel(const grove_kv4_attn_params p, const int shift) {
-  constexpr int NK = HD / 32, NJ = HD / 16, CG = CT < 2 ? CT : 2;  // CG tiles of columns hand their outputs through LDS at a time
+__global__ __launch_bounds__(256, kv4_waves(HD, CT)) void kv4_attn_kernel(const grove_kv4_attn_params p, const int shift) {
+  constexpr int NK = HD / 32, NJ = HD / 16, CG = HD == 256 || CT < 2 ? 1 : 2;  // CG tiles of columns hand their outputs through LDS at a time
+  constexpr bool QL = kv4_q_lds(HD, CT);
   constexpr int S = kv4_slots(HD, CT), BYTES = kv4_bytes(HD), OPS = kv4_ops(HD), PART = kv4_part(HD);
-  static_assert(4 * S * BYTES >= (int)sizeof(float) * 4 * 16 * CG * (HD + 4), "the outputs pass through the rings' memory");
+  static_assert(kv4_lds(HD, CT) >= (int)sizeof(float) * 4 * 16 * CG * (HD + 4), "the outputs pass through the rings' memory");
   extern __shared__ __attribute__((aligned(1024))) char smem[];
   __shared__ float s_m[4][16 * CT], s_l[4][16 * CT], s_c[4][16 * CT];
   float(*s_o)[16 * CG][HD + 4] = (float(*)[16 * CG][HD + 4])smem;
@@ -305,11 +311,11 @@ __global__ __launch_bounds__(256, KV4_WAVES(HD, CT)) void kv4_attn_kernel(const 
   const int tiles = (seen_any + 31) >> 5, per = (tiles + p.n_split - 1) / p.n_split, tile0 = sp * per, tile1 = min(tiles, tile0 + per);
 
   // the columns' queries: asked for after the page numbers and before the first tiles, used when those are on their way
-  bf16x8_t q[CT][NK];
+  bf16x8_t q[QL ? 1 : CT][NK];  // (QL: of the column tile that this wave puts into LDS)
   auto ask_q = [&]() {
 #pragma unroll
-    for (int ct = 0; ct < CT; ++ct) {
-      const int c = col0 + ct * 16 + n16, i = c / G;
+    for (int ct = 0; ct < (QL ? 1 : CT); ++ct) {
+      const int c = col0 + (QL ? w : ct) * 16 + n16, i = c / G;
       const bf16_raw* x = (const bf16_raw*)p.q + (t0 + i) * p.sq_row + (int64_t)(hk * G + c - i * G) * p.sq_head + 8 * h;
 #pragma unroll
       for (int t = 0; t < NK; ++t) {
@@ -319,26 +325,45 @@ __global__ __launch_bounds__(256, KV4_WAVES(HD, CT)) void kv4_attn_kernel(const 
       }
     }
   };
-  float qs[CT], ref[CT], over[CT], l[CT], cst[CT];  // ref: taken off the scores; over: ref + 24, or -inf before the column's first key
-  int lim[CT];
+  float qs[QL ? 1 : CT], ref[CT], l[CT], cst[CT];  // ref: taken off the scores, -inf before the column's first key
   const float a2 = p.alpha * 1.44269504088896340736f;
+  char* q_lds = smem + 4 * S * BYTES;
   auto use_q = [&]() {
 #pragma unroll
-    for (int ct = 0; ct < CT; ++ct) {
-      const int c = col0 + ct * 16 + n16, i = c / G;
+    for (int ct = 0; ct < (QL ? 1 : CT); ++ct) {
       float sum = 0.f;
 #pragma unroll
       for (int t = 0; t < NK; ++t) {
         const u32x4_t r = __builtin_bit_cast(u32x4_t, q[ct][t]);
 #pragma unroll
         for (int e = 0; e < 4; ++e) sum += bf_lo(r[e]) + bf_hi(r[e]);
+        if (QL && w < CT) *(u32x4_t*)(q_lds + ((w * NK + t) * 64 + lane) * 16) = r;
       }
       sum += __shfl_xor(sum, 16, 64);
       sum += __shfl_xor(sum, 32, 64);
       qs[ct] = sum * a2;
-      lim[ct] = c < cols ? base + i : 0;
-      over[ct] = NEG;
-      ref[ct] = 0.f;
+      if (QL && w < CT && h == 0) ((float*)(q_lds + CT * NK * 1024))[w * 16 + n16] = qs[ct];
+    }
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) ref[ct] = NEG;
+    if constexpr (QL) __syncthreads();
+  };
+  const unsigned q_at = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)q_lds + lane * 16;
+  const unsigned qs_at = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)q_lds + CT * NK * 1024 + n16 * 4;
+  auto q_of = [&](int ct, bf16x8_t (&f)[NK], float& sum) {
+    if constexpr (QL) {
+      asm volatile("ds_read_b32 %0, %1\n\ts_waitcnt lgkmcnt(0)" : "=&v"(sum) : "v"(qs_at + ct * 64) : "memory");
+      const unsigned at = q_at + ct * NK * 1024;
+#pragma unroll
+      for (int t = 0; t < NK; t += 4)
+        asm volatile("ds_read_b128 %0, %4 offset:%5\n\tds_read_b128 %1, %4 offset:%6\n\tds_read_b128 %2, %4 offset:%7\n\tds_read_b128 %3, %4 offset:%8\n\t"
+                     "s_waitcnt lgkmcnt(0)"
+                     : "=&v"(f[t]), "=&v"(f[t + 1]), "=&v"(f[t + 2]), "=&v"(f[t + 3])
+                     : "v"(at), "n"(t * 1024), "n"(t * 1024 + 1024), "n"(t * 1024 + 2048), "n"(t * 1024 + 3072) : "memory");
+    } else {
+#pragma unroll
+      for (int t = 0; t < NK; ++t) f[t] = q[ct][t];
+      sum = qs[ct];
     }
   };
   // page numbers by scalar loads (the constant address space), asked for one tile ahead of their use
@@ -396,7 +421,19 @@ __global__ __launch_bounds__(256, KV4_WAVES(HD, CT)) void kv4_attn_kernel(const 
   f32x4_t acc[CT][NJ];
   int tile, from;
   float z[CT][8], top[CT];
-  auto run = [&]() -> bool {  // false: left at a tile, with its scores, for new references
+  auto raise = [&]() -> bool {  // new references for the columns whose scores passed theirs; true: something was summed with an old one
+    bool again = false;
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+      float t = fmaxf(top[ct], __shfl_xor(top[ct], 16, 64));
+      t = fmaxf(t, __shfl_xor(t, 32, 64));
+      const bool up = t - 24.f > ref[ct];
+      again |= up && ref[ct] != NEG;  // (a column's first keys leave nothing to do again)
+      ref[ct] = up ? t : ref[ct];
+    }
+    return __any(again);
+  };
+  auto run = [&]() -> int {  // 0: done, 1: to be started again, 2: left at a tile for new references
     while (tile < tile1) {
       if (ahead - tile == 4 * (S - 1)) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(OPS * (S - 2)) : "memory");  // the tiles behind this one may be on their way
       else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");                                                  // the last ones
@@ -411,24 +448,33 @@ __global__ __launch_bounds__(256, KV4_WAVES(HD, CT)) void kv4_attn_kernel(const 
         for (int t = 0; t < NK; ++t) kf[t] = frag(code_pair(T.k[u][t], 0, kc), code_pair(T.k[u][t], 1, kc), code_pair(T.k[u][t], 2, kc), code_pair(T.k[u][t], 3, kc));
 #pragma unroll
         for (int ct = 0; ct < CT; ++ct) {
+          bf16x8_t qf[NK];
+          float qsum;
+          q_of(ct, qf, qsum);
           f32x4_t raw = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int t = 0; t < NK; ++t) raw = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[t], q[ct][t], raw, 0, 0, 0);
+          for (int t = 0; t < NK; ++t) raw = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[t], qf[t], raw, 0, 0, 0);
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const float s = bf_lo(T.ks[u][i]), mn = bf_hi(T.ks[u][i]);
-            z[ct][4 * u + i] = fmaf(raw[i], a2 * s, fmaf(-16.f, s, mn) * qs[ct]);
+            z[ct][4 * u + i] = fmaf(raw[i], a2 * s, fmaf(-16.f, s, mn) * qsum);
           }
         }
       }
       const unsigned miss = bad >> (2 * from) & 3;
       const bool masked = ((tile + 1) * 32 > seen_all) | (miss != 0);
-      auto sees = [&](int ct, int i) { return (tile * 32 + 16 * (i >> 2) + 4 * h + (i & 3) < lim[ct]) & ((miss >> (i >> 2) & 1) == 0); };
+      auto limit = [&](int ct) {  // of keys that a column sees
+        const int c = col0 + ct * 16 + n16;
+        return c < cols ? base + c / G : 0;
+      };
+      auto sees = [&](int lim, int i) { return (tile * 32 + 16 * (i >> 2) + 4 * h + (i & 3) < lim) & ((miss >> (i >> 2) & 1) == 0); };
       if (masked) {
 #pragma unroll
-        for (int ct = 0; ct < CT; ++ct)
+        for (int ct = 0; ct < CT; ++ct) {
+          const int lim = limit(ct);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) z[ct][i] = sees(ct, i) ? z[ct][i] : NEG;
+          for (int i = 0; i < 8; ++i) z[ct][i] = sees(lim, i) ? z[ct][i] : NEG;
+        }
       }
       bool grow = false;
 #pragma unroll
@@ -436,31 +482,43 @@ __global__ __launch_bounds__(256, KV4_WAVES(HD, CT)) void kv4_attn_kernel(const 
         top[ct] = z[ct][0];
 #pragma unroll
         for (int i = 1; i < 8; ++i) top[ct] = fmaxf(top[ct], z[ct][i]);
-        grow |= top[ct] > over[ct];
+        grow |= top[ct] - 24.f > ref[ct];
       }
-      if (__any(grow)) return false;
+      if (__any(grow)) {
+        if constexpr (HD * CT >= 512) return 2;  // (outside of the loop: inside it the paths' joined registers do not fit)
+        if (raise()) return 1;
+      }
       if (ahead < tile1) issue();
       ring_read<HD, 2 * PART, 4 * PART + 128>(at_values, at_scales, T.v, T.vs);
       if (masked) {  // 0 times a scale that is no number would reach the columns that do not see its row: it goes, and those that see it become NaN
+        unsigned odd = 0;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           const unsigned sm = T.vs[i >> 2][i & 3];
-          const bool odd = ((sm & 0x7f80u) == 0x7f80u) | ((sm & 0x7f800000u) == 0x7f800000u);
+          const bool is = ((sm & 0x7f80u) == 0x7f80u) | ((sm & 0x7f800000u) == 0x7f800000u);
+          odd |= is ? 1u << i : 0u;
+          T.vs[i >> 2][i & 3] = is ? 0u : sm;
+        }
+        if (__any(odd != 0)) {
 #pragma unroll
-          for (int ct = 0; ct < CT; ++ct) l[ct] = odd & sees(ct, i) ? NAN : l[ct];
-          T.vs[i >> 2][i & 3] = odd ? 0u : sm;
+          for (int ct = 0; ct < CT; ++ct) {
+            const int lim = limit(ct);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) l[ct] = ((odd >> i & 1) != 0) & sees(lim, i) ? NAN : l[ct];
+          }
         }
       }
       bf16x8_t hi[CT], lo[CT];
 #pragma unroll
       for (int ct = 0; ct < CT; ++ct) {
+        const float off = ref[ct] == NEG ? 0.f : ref[ct];
         unsigned a[4], c[4];
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
           float ps[4];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const float e = __builtin_amdgcn_exp2f(z[ct][4 * u + i] - ref[ct]);
+            const float e = __builtin_amdgcn_exp2f(z[ct][4 * u + i] - off);
             const float s = bf_lo(T.vs[u][i]), mn = fmaf(-16.f, s, bf_hi(T.vs[u][i]));
             l[ct] += e;
             ps[i] = e * s;
@@ -493,46 +551,37 @@ __global__ __launch_bounds__(256, KV4_WAVES(HD, CT)) void kv4_attn_kernel(const 
       tile += 4;
       from = from == S - 1 ? 0 : from + 1;
     }
-    return true;
+    return 0;
   };
-  bool first = true, again;
-  ahead = tile0 + w;
-  if (ahead < tile1) ask_pages();
-  ask_q();
-  do {
-    again = false;
-    tile = ahead;
+  auto start = [&]() {
+    tile = ahead = tile0 + w;
     to = from = 0;
     bad = 0;
+    if (ahead < tile1) ask_pages();
+  };
+  auto fill = [&]() {  // (rolled: what a block runs once is fetched cold, and its length counts)
 #pragma unroll 1
-    for (int i = 0; i < S - 1 && ahead < tile1; ++i) issue();  // (rolled: what a block runs once is fetched cold, and its length counts)
-    if (first) use_q();
-    first = false;
+    for (int i = 0; i < S - 1 && ahead < tile1; ++i) issue();
+  };
+  start();
+  ask_q();
+  fill();
+  use_q();
+  while (true) {
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
       l[ct] = cst[ct] = 0.f;
 #pragma unroll
       for (int j = 0; j < NJ; ++j) acc[ct][j] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
     }
-    while (!run()) {
-#pragma unroll
-      for (int ct = 0; ct < CT; ++ct) {
-        float t = fmaxf(top[ct], __shfl_xor(top[ct], 16, 64));
-        t = fmaxf(t, __shfl_xor(t, 32, 64));
-        const bool up = t > over[ct];
-        again |= up && over[ct] != NEG;  // (a column's first keys leave nothing to do again)
-        ref[ct] = up ? t : ref[ct];
-        over[ct] = up ? t + 24.f : over[ct];
-      }
-      again = __any(again);
-      if (again) {
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the tiles in flight land before their slots are asked for again
-        ahead = tile0 + w;
-        ask_pages();
-        break;
-      }
+    int left;
+    while ((left = run()) == 2 && !raise()) {
     }
-  } while (again);
+    if (left == 0) break;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the tiles in flight land before their slots are asked for again
+    start();
+    fill();
+  }
 
   // the four waves' results: one maximum per column, the outputs through LDS
 #pragma unroll
@@ -542,7 +591,7 @@ __global__ __launch_bounds__(256, KV4_WAVES(HD, CT)) void kv4_attn_kernel(const 
     cst[ct] += __shfl_xor(cst[ct], 16, 64);
     cst[ct] += __shfl_xor(cst[ct], 32, 64);
     if (h == 0) {
-      s_m[w][ct * 16 + n16] = over[ct] == NEG ? NEG : ref[ct];
+      s_m[w][ct * 16 + n16] = ref[ct];
       s_l[w][ct * 16 + n16] = l[ct];
       s_c[w][ct * 16 + n16] = cst[ct];
     }
@@ -734,7 +783,7 @@ extern "C" int grove_kv4_attn(const grove_kv4_attn_params* p, void* stream) {
   const dim3 grid((unsigned)p->n_split, (unsigned)(chunks * p->kv), (unsigned)p->requests);
 #define RUN(HD, CT)                                                                                                                  \
   do {                                                                                                                               \
-    constexpr int lds = 4 * kv4_slots(HD, CT) * kv4_bytes(HD);                                                                       \
+    constexpr int lds = kv4_lds(HD, CT);                                                                                             \
     if (lds > 64 * 1024) hipFuncSetAttribute((const void*)kv4_attn_kernel<HD, CT>, hipFuncAttributeMaxDynamicSharedMemorySize, lds);                      \
     hipLaunchKernelGGL((kv4_attn_kernel<HD, CT>), grid, dim3(256), lds, (hipStream_t)stream, *p, shift);               \
   } while (0)

@@ -1438,11 +1438,12 @@ def _kv4_split(pairs, max_len, cols, hd):
     """Blocks to which the keys of a (request, key / value head) pair are dealt. A CU streams some 22 GB/s whatever it has in flight, so the 256 of
     them are to be filled as soon as a block's four waves have three tiles of 32 keys (32 pairs of 703 keys: 10.6 us in one block each, 8.6 in
     eight, 10 in sixteen); beyond that ragged lengths want some 2048 blocks as long as a block keeps 1024 keys (256 pairs of up to 32768 keys: 263
-    us in one block each, 128 in 8, 187 in 64), or 2048 per tile of 16 columns where there are several (512 pairs of up to 4096 keys under 32
-    columns: 70 us in one block each, 74 in 2, 101 in 8): behind that a block's start and its partial results count."""
+    us in one block each, 128 in 8, 187 in 64). Where several tiles of 16 columns share the keys, half as many blocks of twice as many keys (256
+    pairs of up to 8192 keys under 64 columns: 166 us in one block each, 107 in 4, 118 in 8): a block's start and its partial results count more."""
     ct = 1 if cols <= 16 else 2 if cols <= 32 or hd == 256 else 4
     pairs *= max(1, -(-cols // (16 * ct)))
-    return max(1, min(64, max(min(256 // pairs, max_len // 96), min(2048 // pairs, max_len // (1024 if ct == 1 else 2048 * ct)))))
+    most, least = (2048, 1024) if ct == 1 else (1024, 16 * max(hd, 128))
+    return max(1, min(64, max(min(256 // pairs, max_len // 96), min(most // pairs, max_len // least))))
 
 
 def kv4_attn(q, cache, table, kv_len, cu_q, max_q, alpha, *, max_len=None, out=None):
