@@ -351,20 +351,12 @@ __global__ __launch_bounds__(256, kv4_waves(HD, CT)) void kv4_attn_kernel(const 
   const unsigned q_at = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)q_lds + lane * 16;
   const unsigned qs_at = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)q_lds + CT * NK * 1024 + n16 * 4;
   auto q_of = [&](int ct, bf16x8_t (&f)[NK], float& sum) {
-    if constexpr (QL) {
-      asm volatile("ds_read_b32 %0, %1\n\ts_waitcnt lgkmcnt(0)" : "=&v"(sum) : "v"(qs_at + ct * 64) : "memory");
-      const unsigned at = q_at + ct * NK * 1024;
-#pragma unroll
-      for (int t = 0; t < NK; t += 4)
-        asm volatile("ds_read_b128 %0, %4 offset:%5\n\tds_read_b128 %1, %4 offset:%6\n\tds_read_b128 %2, %4 offset:%7\n\tds_read_b128 %3, %4 offset:%8\n\t"
-                     "s_waitcnt lgkmcnt(0)"
-                     : "=&v"(f[t]), "=&v"(f[t + 1]), "=&v"(f[t + 2]), "=&v"(f[t + 3])
-                     : "v"(at), "n"(t * 1024), "n"(t * 1024 + 1024), "n"(t * 1024 + 2048), "n"(t * 1024 + 3072) : "memory");
-    } else {
-#pragma unroll
-      for (int t = 0; t < NK; ++t) f[t] = q[ct][t];
-      sum = qs[ct];
-    }
+    const unsigned at = q_at + ct * NK * 1024;
+    static_assert(!QL || NK == 4, "four operands a column tile");
+    asm volatile("ds_read_b128 %0, %5 offset:%7\n\tds_read_b128 %1, %5 offset:%8\n\tds_read_b128 %2, %5 offset:%9\n\tds_read_b128 %3, %5 offset:%10\n\t"
+                 "ds_read_b32 %4, %6\n\ts_waitcnt lgkmcnt(0)"
+                 : "=&v"(f[0]), "=&v"(f[1 % NK]), "=&v"(f[2 % NK]), "=&v"(f[3 % NK]), "=&v"(sum)
+                 : "v"(at), "v"(qs_at + ct * 64), "n"(0), "n"(1024), "n"(2048), "n"(3072) : "memory");
   };
   // page numbers by scalar loads (the constant address space), asked for one tile ahead of their use
   const scalar_ints row = (scalar_ints)(uintptr_t)(p.table + b * p.ld_table);
@@ -440,25 +432,51 @@ __global__ __launch_bounds__(256, kv4_waves(HD, CT)) void kv4_attn_kernel(const 
       const unsigned slot = ring_at + from * BYTES, at_scales = slot + 16 * h;
       const unsigned at_keys = slot + (HD < 128 ? n16 * (HD / 2) + h * (HD / 8) : lane * 16), at_values = slot + lane * (HD < 128 ? HD / 8 : 16);
       ring_read<HD, 0, 4 * PART>(at_keys, at_scales, T.k, T.ks);
+      // One part's operands at a time, both where there is one column tile: unpacked all at once they would take the registers of another wave. The
+      // products of different tiles take turns, so that none waits for the one before it.
+      constexpr int UG = CT == 1 && HD <= 128 ? 2 : 1;
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        __builtin_amdgcn_sched_barrier(0);  // one part's operands at a time: unpacked all at once they would take the registers of a third wave
-        bf16x8_t kf[NK];
+      for (int u0 = 0; u0 < 2; u0 += UG) {
+        __builtin_amdgcn_sched_barrier(0);
+        bf16x8_t kf[UG][NK];
 #pragma unroll
-        for (int t = 0; t < NK; ++t) kf[t] = frag(code_pair(T.k[u][t], 0, kc), code_pair(T.k[u][t], 1, kc), code_pair(T.k[u][t], 2, kc), code_pair(T.k[u][t], 3, kc));
+        for (int u = 0; u < UG; ++u)
 #pragma unroll
-        for (int ct = 0; ct < CT; ++ct) {
-          bf16x8_t qf[NK];
-          float qsum;
-          q_of(ct, qf, qsum);
-          f32x4_t raw = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int t = 0; t < NK; ++t) raw = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[t], qf[t], raw, 0, 0, 0);
+          for (int t = 0; t < NK; ++t) {
+            const unsigned x = T.k[u0 + u][t];
+            kf[u][t] = frag(code_pair(x, 0, kc), code_pair(x, 1, kc), code_pair(x, 2, kc), code_pair(x, 3, kc));
+          }
+        auto score = [&](int ct, int u, const f32x4_t raw, float qsum) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const float s = bf_lo(T.ks[u][i]), mn = bf_hi(T.ks[u][i]);
             z[ct][4 * u + i] = fmaf(raw[i], a2 * s, fmaf(-16.f, s, mn) * qsum);
           }
+        };
+        if constexpr (QL) {
+#pragma unroll
+          for (int ct = 0; ct < CT; ++ct) {
+            bf16x8_t qf[NK];
+            float qsum;
+            q_of(ct, qf, qsum);
+            f32x4_t raw = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int t = 0; t < NK; ++t) raw = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[0][t], qf[t], raw, 0, 0, 0);
+            score(ct, u0, raw, qsum);
+          }
+        } else {
+          f32x4_t raw[UG][CT];
+#pragma unroll
+          for (int t = 0; t < NK; ++t)
+#pragma unroll
+            for (int u = 0; u < UG; ++u)
+#pragma unroll
+              for (int ct = 0; ct < CT; ++ct)
+                raw[u][ct] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[u][t], q[ct][t], t ? raw[u][ct] : (f32x4_t){0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+#pragma unroll
+          for (int u = 0; u < UG; ++u)
+#pragma unroll
+            for (int ct = 0; ct < CT; ++ct) score(ct, u0 + u, raw[u][ct], qs[ct]);
         }
       }
       const unsigned miss = bad >> (2 * from) & 3;
@@ -534,19 +552,23 @@ __global__ __launch_bounds__(256, kv4_waves(HD, CT)) void kv4_attn_kernel(const 
         lo[ct] = frag(c[0], c[1], c[2], c[3]);
       }
 #pragma unroll
-      for (int j = 0; j < NJ; ++j) {
-        if ((j & 1) == 0) __builtin_amdgcn_sched_barrier(0);
-        bf16x8_t vf;
-        if constexpr (HD == 32) vf = frag(code_pair(T.v[0][0], j, kc), code_pair(T.v[0][0], j + 2, kc), code_pair(T.v[1][0], j, kc), code_pair(T.v[1][0], j + 2, kc));
-        else {
-          const int o = (j >> 2) * 2, jn = j & 3;
-          vf = frag(code_pair(T.v[0][o], jn, kc), code_pair(T.v[0][o + 1], jn, kc), code_pair(T.v[1][o], jn, kc), code_pair(T.v[1][o + 1], jn, kc));
+      for (int j = 0; j < NJ; j += 2) {
+        __builtin_amdgcn_sched_barrier(0);
+        bf16x8_t vf[2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          if constexpr (HD == 32) vf[k] = frag(code_pair(T.v[0][0], k, kc), code_pair(T.v[0][0], k + 2, kc), code_pair(T.v[1][0], k, kc), code_pair(T.v[1][0], k + 2, kc));
+          else {
+            const int o = (j >> 2) * 2, jn = (j & 3) + k;
+            vf[k] = frag(code_pair(T.v[0][o], jn, kc), code_pair(T.v[0][o + 1], jn, kc), code_pair(T.v[1][o], jn, kc), code_pair(T.v[1][o + 1], jn, kc));
+          }
         }
 #pragma unroll
-        for (int ct = 0; ct < CT; ++ct) {
-          acc[ct][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, hi[ct], acc[ct][j], 0, 0, 0);
-          acc[ct][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, lo[ct], acc[ct][j], 0, 0, 0);
-        }
+        for (int part = 0; part < 2; ++part)
+#pragma unroll
+          for (int k = 0; k < 2; ++k)
+#pragma unroll
+            for (int ct = 0; ct < CT; ++ct) acc[ct][j + k] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf[k], part ? lo[ct] : hi[ct], acc[ct][j + k], 0, 0, 0);
       }
       tile += 4;
       from = from == S - 1 ? 0 : from + 1;
