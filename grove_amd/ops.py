@@ -7,6 +7,7 @@ Tensors are bf16 unless stated; every function launches on torch's current strea
 import ctypes as C
 import math
 import os
+import struct
 from typing import NamedTuple
 
 import torch
@@ -1187,23 +1188,33 @@ def _refuse(what, msg):
     raise RuntimeError(f"{what}: {msg}")
 
 
+def _packer(params):
+    """struct.pack for a ctypes params struct: a third of the time of filling the ctypes object."""
+    code = {_lib.c_vp: "P", _lib.c_i64: "q", _lib.c_i32: "i", _lib.c_f32: "f"}
+    pack = struct.Struct("@" + "".join(code[t] for _, t in params._fields_) + "0P")
+    assert pack.size == C.sizeof(params), params
+    return pack.pack
+
+
 _entries = {}
 
 
 def _launch(name, params, *ts):
     """Calls grove_<name>. Every tensor must be on the CURRENT device: the launch goes to its current stream, wherever the tensors are."""
-    if ts[0].get_device() < 0:
+    cur = ts[0].get_device()
+    if cur < 0:
         raise RuntimeError(f"{name}: grove_amd ops need device tensors (no CPU fallback exists)")
-    cur = torch._C._cuda_getDevice()
+    if cur != torch._C._cuda_getDevice():
+        _refuse(name, f"a tensor is on {ts[0].device}, the current device is cuda:{torch.cuda.current_device()}")
     for t in ts:
         if t is not None and t.get_device() != cur:
-            _refuse(name, f"a tensor is on {t.device}, the current device is cuda:{cur}")
+            _refuse(name, f"a tensor is on {t.device}, another on cuda:{cur}")
     fn = _entries.get(name)
     if fn is None:
         fn = getattr(_lib.lib(), "grove_" + name)
         fn.argtypes = [C.c_void_p, C.c_void_p]
         _entries[name] = fn
-    rc = fn(C.byref(params), torch._C._cuda_getCurrentRawStream(cur))
+    rc = fn(params, torch._C._cuda_getCurrentRawStream(cur))
     if rc:
         _lib.check(rc, "grove_" + name)
 
@@ -1213,8 +1224,11 @@ def _need_device(what, t):
         raise RuntimeError(f"{what}: grove_amd ops need device tensors (no CPU fallback exists)")
 
 
+_i32, _f32 = torch.int32, torch.float32
+
+
 def _lens(what, name, t, n):
-    if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous():
+    if t.dtype != _i32 or t.shape != (n,) or not t.is_contiguous():
         _refuse(what, f"{name} must be contiguous int32 [{n}]")
 
 
@@ -1239,6 +1253,10 @@ def _own_elements(t):
             return False
         at = s * n
     return True
+
+
+_pack_rotary, _pack_pagetables, _pack_verifydrafts = _packer(_lib.RotaryParams), _packer(_lib.PageTablesParams), _packer(_lib.VerifyDraftsParams)
+_pack_kv4append, _pack_kv4read, _pack_kv4attn = _packer(_lib.Kv4AppendParams), _packer(_lib.Kv4ReadParams), _packer(_lib.Kv4AttnParams)
 
 
 class RotaryPlan(NamedTuple):
@@ -1302,7 +1320,7 @@ def rotary(x, pos, plan, *, backward=False, out=None):
     _lens(what, "pos", pos, rows)
     if out is None:
         _need_device(what, x)
-        out = torch.empty((rows, heads, hd), dtype=dt, device=x.device)
+        out = x.new_empty((rows, heads, hd))
         yr, yh = heads * hd, hd
     else:
         if out.shape != x.shape or out.dtype != dt or (out.stride(2) != 1 and hd > 1 and out.numel()):
@@ -1312,7 +1330,7 @@ def rotary(x, pos, plan, *, backward=False, out=None):
         yr, yh = out.stride(0), out.stride(1)
         if not (out.data_ptr() == x.data_ptr() and yr == sr and yh == sh) and not _apart(out, x):
             _refuse(what, "out overlaps x and is not the same view")
-    p = _lib.RotaryParams(x.data_ptr(), out.data_ptr(), pos.data_ptr(), f.data_ptr(), sr, sh, yr, yh, rows, heads, hd, 2 * f.shape[0],
+    p = _pack_rotary(x.data_ptr(), out.data_ptr(), pos.data_ptr(), f.data_ptr(), sr, sh, yr, yh, rows, heads, hd, 2 * f.shape[0],
                           interleaved, backward, dt == torch.float32, mscale)
     _launch(what, p, x, pos, f, out)
     return out
@@ -1355,10 +1373,10 @@ def page_tables(ctx_len, new_len, table, held, free, page_size, rows):
         if a < t1 and a + 4 * n > t0:
             _refuse(what, "table overlaps an input")
     _need_device(what, table)
-    o = torch.empty(3 * B + 2 + 2 * rows, dtype=torch.int32, device=table.device)  # one allocation for the six results
+    o = table.new_empty(3 * B + 2 + 2 * rows)  # one allocation for the six results
     o0 = o.data_ptr()
     o1, o2, o3, o4, o5 = o0 + 4 * B, o0 + 8 * B + 4, o0 + 8 * B + 4 + 4 * rows, o0 + 8 * B + 4 + 8 * rows, o0 + 12 * B + 4 + 8 * rows
-    p = _lib.PageTablesParams(*at, t0, o0, o1, o2, o3, o4, o5, ld, B, most, page_size, rows, free.shape[0])
+    p = _pack_pagetables(*at, t0, o0, o1, o2, o3, o4, o5, ld, B, most, page_size, rows, free.shape[0])
     _launch(what, p, table, ctx_len, new_len, held, free)
     return PageStep(*o.split_with_sizes((B, B + 1, rows, rows, B, 1)))
 
@@ -1414,7 +1432,7 @@ def kv4_append(k, v, cache, slots):
             _refuse(what, "an input lies in the cache")
     kr, kh, _ = k.stride()
     vr, vh, _ = v.stride()
-    _launch(what, _lib.Kv4AppendParams(kp, vp, c0, s0, sp, kr, kh, vr, vh, rows, kv, hd, P, pages), k, v, codes, scales, slots)
+    _launch(what, _pack_kv4append(kp, vp, c0, s0, sp, kr, kh, vr, vh, rows, kv, hd, P, pages), k, v, codes, scales, slots)
 
 
 def kv4_read(cache, slots, out_dtype=bf16):
@@ -1429,7 +1447,7 @@ def kv4_read(cache, slots, out_dtype=bf16):
     codes, scales = cache
     k = torch.empty((rows, kv, hd), dtype=out_dtype, device=slots.device)
     v = torch.empty((rows, kv, hd), dtype=out_dtype, device=slots.device)
-    p = _lib.Kv4ReadParams(codes.data_ptr(), scales.data_ptr(), slots.data_ptr(), k.data_ptr(), v.data_ptr(), rows, kv, hd, P, pages, out_dtype == torch.float32)
+    p = _pack_kv4read(codes.data_ptr(), scales.data_ptr(), slots.data_ptr(), k.data_ptr(), v.data_ptr(), rows, kv, hd, P, pages, out_dtype == torch.float32)
     _launch(what, p, slots, codes, scales)
     return k, v
 
@@ -1472,7 +1490,7 @@ def kv4_attn(q, cache, table, kv_len, cu_q, max_q, alpha, *, max_len=None, out=N
     fresh = out is None
     if fresh:
         _need_device(what, q)
-        out = torch.empty((rows, heads * hd), dtype=bf16, device=q.device)
+        out = q.new_empty((rows, heads * hd))
         orow = heads * hd
     else:
         if out.dtype != bf16 or out.dim() != 2 or out.shape[0] != rows or out.shape[1] != heads * hd or (out.stride(1) != 1 and out.numel()) or not _own_elements(out):
@@ -1487,8 +1505,8 @@ def kv4_attn(q, cache, table, kv_len, cu_q, max_q, alpha, *, max_len=None, out=N
         qr, qh = heads * hd, hd
     n_split = _kv4_split(B * kv, most * P if max_len is None else max_len, min(max_q, rows) * (heads // kv), hd)
     # the joined splits' workspace: from the allocator at every call, so that calls on other streams and captured graphs have their own
-    partial = torch.empty(rows * heads * n_split * (hd + 2), dtype=torch.float32, device=q.device) if n_split > 1 else None
-    p = _lib.Kv4AttnParams(q.data_ptr(), codes.data_ptr(), scales.data_ptr(), table.data_ptr(), kv_len.data_ptr(), cu_q.data_ptr(), out.data_ptr(),
+    partial = q.new_empty(rows * heads * n_split * (hd + 2), dtype=_f32) if n_split > 1 else None
+    p = _pack_kv4attn(q.data_ptr(), codes.data_ptr(), scales.data_ptr(), table.data_ptr(), kv_len.data_ptr(), cu_q.data_ptr(), out.data_ptr(),
                            0 if partial is None else partial.data_ptr(), qr, qh, orow, max(table.stride(0), most), B, heads, kv, hd, P, pages, most,
                            rows, max_q, n_split, fresh, alpha)
     _launch(what, p, q, codes, scales, table, kv_len, cu_q, out)
@@ -1523,10 +1541,12 @@ def verify_drafts(draft, q, p, u, pick, count=None):
     if count is not None:
         _lens(what, "count", count, B)
     _need_device(what, p)
-    tokens = torch.empty((B, K + 1), dtype=torch.int32, device=p.device)
-    accepted = torch.empty(B, dtype=torch.int32, device=p.device)
-    partial = torch.empty(B * min(1024, -(-V // 1024)), dtype=torch.float64, device=p.device) if V > _VERIFY_SPLIT and 0 < B < 512 else None
-    a = _lib.VerifyDraftsParams(draft.data_ptr(), qp, p.data_ptr(), u.data_ptr(), pick.data_ptr(), 0 if count is None else count.data_ptr(), tokens.data_ptr(),
-                                accepted.data_ptr(), 0 if partial is None else partial.data_ptr(), qb, qr, p.stride(0), p.stride(1), B, K, V, dt == bf16)
+    n = B * min(1024, -(-V // 1024)) if V > _VERIFY_SPLIT and B < 512 else 0
+    o = draft.new_empty(2 * n + B * (K + 2))  # one allocation: the sums' workspace (f64), the tokens, the numbers accepted
+    o0 = o.data_ptr()
+    t0 = o0 + 8 * n
+    a = _pack_verifydrafts(draft.data_ptr(), qp, p.data_ptr(), u.data_ptr(), pick.data_ptr(), 0 if count is None else count.data_ptr(), t0, t0 + 4 * B * (K + 1),
+                           o0 if n else 0, qb, qr, p.stride(0), p.stride(1), B, K, V, dt == bf16)
     _launch(what, a, p, draft, q if qp else None, u, pick, count)
-    return tokens, accepted
+    _, tokens, accepted = o.split_with_sizes((2 * n, B * (K + 1), B))
+    return tokens.view(B, K + 1), accepted
