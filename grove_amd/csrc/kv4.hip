@@ -306,7 +306,7 @@ __global__ __launch_bounds__(256, kv4_waves(HD, CT)) void kv4_attn_kernel(const 
   const int cols = min(n, p.max_q) * G, col0 = cc * 16 * CT;
   if (col0 >= cols) return;
   const int64_t room = (int64_t)p.max_pages << shift;
-  const int base = (int)min((int64_t)kv_len, room) - n + 1;  // token i sees base + i keys
+  const int base = (int)min((int64_t)max(kv_len, 0), room) - n + 1;  // token i sees base + i keys
   const int seen_all = max(0, base + col0 / G), seen_any = max(0, base + (min(cols, col0 + 16 * CT) - 1) / G);
   const int tiles = (seen_any + 31) >> 5, per = (tiles + p.n_split - 1) / p.n_split, tile0 = sp * per, tile1 = min(tiles, tile0 + per);
 
@@ -793,7 +793,7 @@ extern "C" int grove_kv4_attn(const grove_kv4_attn_params* p, void* stream) {
   GROVE_CHECK(p->q && p->codes && p->scales && p->table && p->kv_len && p->cu_q && p->out, GROVE_E_SHAPE, "kv4_attn: null pointer");
   GROVE_CHECK(((uintptr_t)p->codes & 15) == 0 && ((uintptr_t)p->scales & 15) == 0, GROVE_E_ALIGN, "kv4_attn: the cache must be 16-byte aligned");
   GROVE_CHECK(p->n_split >= 1 && p->n_split <= 64 && (p->n_split == 1 || p->partial), GROVE_E_WORKSPACE, "kv4_attn: 1 to 64 splits, more than one with a workspace");
-  GROVE_CHECK((int64_t)p->max_pages * p->page <= 0x7fffffff, GROVE_E_SHAPE, "kv4_attn: the table holds more than 2^31 tokens");
+  GROVE_CHECK((int64_t)p->max_pages * p->page <= 1 << 30, GROVE_E_SHAPE, "kv4_attn: a row of the table holds more than 2^30 tokens");
   const int shift = __builtin_ctz((unsigned)p->page);
   GROVE_CHECK(((uintptr_t)p->q & 15) == 0 && p->sq_row % 8 == 0 && p->sq_head % 8 == 0 && ((uintptr_t)p->out & 3) == 0 && p->so_row % 2 == 0, GROVE_E_ALIGN,
               "kv4_attn: q must be aligned to 16 bytes and out to 4, their strides too");

@@ -1484,14 +1484,16 @@ def kv4_attn(q, cache, table, kv_len, cu_q, max_q, alpha, *, max_len=None, out=N
     _lens(what, "cu_q", cu_q, B + 1)
     if B > 65535 or max_q < 0:
         _refuse(what, "at most 65535 requests, max_q must not be negative")
-    if most * P >= 2 ** 31:
-        _refuse(what, "the table holds more than 2^31 tokens")
+    if most * P > 2 ** 30:
+        _refuse(what, "a row of the table holds more than 2^30 tokens")
     codes, scales = cache
     fresh = out is None
     if fresh:
         _need_device(what, q)
         out = q.new_empty((rows, heads * hd))
         orow = heads * hd
+        if max_q == 0:
+            out.zero_()
     else:
         if out.dtype != bf16 or out.dim() != 2 or out.shape[0] != rows or out.shape[1] != heads * hd or (out.stride(1) != 1 and out.numel()) or not _own_elements(out):
             _refuse(what, f"out must be bf16 [{rows}, {heads * hd}], its rows contiguous and apart")

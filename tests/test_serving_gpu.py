@@ -499,6 +499,46 @@ def test_attn_lengths_past_the_table(dev):
     assert torch.equal(r[0], out[0])
 
 
+@pytest.mark.parametrize("lens,H,kv,hd,P", [([300, 33], 8, 2, 64, 16), ([500], 4, 4, 128, 32), ([130, 1, 0], 16, 2, 128, 64), ([90], 4, 1, 256, 16)])
+def test_attn_whole_prompts(dev, lens, H, kv, hd, P):
+    """Every token of the cache is new: the causal triangle from its first row, many column chunks."""
+    check_attn(dev, lens, lens, H, kv, hd, P, seed=81)
+
+
+def test_attn_nothing(dev):
+    """No rows; rows of nobody with max_q 0; lengths below zero."""
+    from grove_amd import ops
+    c, q, cu, kv_len, out = check_attn(dev, [20, 30], [2, 1], 4, 2, 64, 16, seed=91)
+    none = torch.zeros(3, dtype=i32, device=dev)
+    assert ops.kv4_attn(q[:0].to(dev), c.cache, c.table, kv_len, none, 0, 1.0).shape == (0, 256)
+    assert (ops.kv4_attn(q.to(dev), c.cache, c.table, kv_len, none, 0, 1.0) == 0).all()
+    assert (ops.kv4_attn(q.to(dev), c.cache, c.table, kv_len, none, 3, 1.0) == 0).all()
+    assert (ops.kv4_attn(q.to(dev), c.cache, c.table, torch.full_like(kv_len, -2 ** 31), cu, 2, 1.0) == 0).all()
+    assert torch.equal(ops.kv4_attn(q.to(dev), c.cache, c.table, kv_len, cu, 2, 0.125), out)
+
+
+def test_attn_offsets_past_32_bits(dev):
+    """The last pages of a cache of more than 4 GiB of codes."""
+    from grove_amd import ops
+    kv, hd, P, pages, L = 8, 128, 64, 70000, 150
+    cache = ops.KV4Cache(torch.empty(pages, 2, kv, P * hd // 2, dtype=torch.uint8, device=dev), torch.empty(pages, 2, kv, P, 2, dtype=bf16, device=dev))
+    table = torch.tensor([[69999, 3, 69997]], dtype=i32, device=dev)
+    slots = (table[0, torch.arange(L, device=dev) // P] * P + torch.arange(L, device=dev) % P).to(i32)
+    k, v = (torch.randn(L, kv, hd, generator=gen(s)).to(bf16) for s in (1, 2))
+    ops.kv4_append(k.to(dev), v.to(dev), cache, slots)
+    c = Paged.__new__(Paged)
+    c.kv, c.lens, c.k, c.v, c.size = kv, [L], [], [], []
+    for x, got, store in zip((k, v), ops.kv4_read(cache, slots, f32), (c.k, c.v)):
+        codes, s, m = quant_ref(x)
+        assert torch.equal(got.cpu(), (m + codes * s).to(f32))
+        store.append(got.cpu().to(f64))
+        c.size.append(float((31 * s).max() + got.abs().max()))
+    q = torch.randn(2, 32, hd, generator=gen(3)).to(bf16)
+    out = ops.kv4_attn(q.to(dev), cache, table, torch.tensor([L], dtype=i32, device=dev), torch.tensor([0, 2], dtype=i32, device=dev), 2, hd ** -0.5)
+    ref, tol = c.ref(q, [2], hd ** -0.5)
+    within(out, ref, tol)
+
+
 def test_attn_same_bits_every_time(dev):
     from grove_amd import ops
     c, q, cu, kv_len, out = check_attn(dev, [7000, 30], [2, 1], 8, 2, 128, 64, seed=51)

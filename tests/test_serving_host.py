@@ -110,6 +110,7 @@ def test_attn_refusals():
     refused("out must", ops.kv4_attn, q, c, t, n, cu, 2, 1.0, out=torch.zeros(1, 256, dtype=bf16).expand(3, 256))
     refused("overlaps", ops.kv4_attn, q, c, t, n, cu, 2, 1.0, out=q.view(3, 256))
     refused("max_q", ops.kv4_attn, q, c, t, n, cu, -1, 1.0)
+    refused("aligned to 4 bytes", ops.kv4_attn, q, c, t, n, cu, 2, 1.0, out=torch.zeros(3, 257, dtype=bf16)[:, 1:])
     refused("device", ops.kv4_attn, q, c, t, n, cu, 2, 1.0)
 
 
@@ -151,6 +152,12 @@ def entry(name, struct, **fields):
     ("grove_kv4_read", _lib.Kv4ReadParams, dict(rows=1, kv=1, hd=64, page=16, pages=1), -1, "null"),
     ("grove_kv4_attn", _lib.Kv4AttnParams, dict(requests=1, rows=1, heads=3, kv=2, hd=64, page=16, pages=1, max_pages=1, ld_table=1, max_q=1), -1, "multiple"),
     ("grove_kv4_attn", _lib.Kv4AttnParams, dict(requests=1, rows=1, heads=2, kv=2, hd=64, page=16, pages=1, max_pages=1, ld_table=1, max_q=1), -1, "null"),
+    ("grove_kv4_attn", _lib.Kv4AttnParams, dict(requests=1, rows=1, heads=2, kv=2, hd=64, page=16, pages=1, max_pages=1 << 27, ld_table=1 << 27, max_q=1, q=64,
+                                                codes=64, scales=64, table=64, kv_len=64, cu_q=64, out=64, n_split=1), -1, "2^30"),
+    ("grove_kv4_attn", _lib.Kv4AttnParams, dict(requests=1, rows=1, heads=2, kv=2, hd=64, page=16, pages=1, max_pages=1, ld_table=1, max_q=1, q=72,
+                                                codes=64, scales=64, table=64, kv_len=64, cu_q=64, out=64, n_split=1), -3, "aligned"),
+    ("grove_kv4_attn", _lib.Kv4AttnParams, dict(requests=1, rows=1, heads=2, kv=2, hd=64, page=16, pages=1, max_pages=1, ld_table=1, max_q=1, q=64,
+                                                codes=64, scales=64, table=64, kv_len=64, cu_q=64, out=64, n_split=2), -4, "workspace"),
     ("grove_verify_drafts", _lib.VerifyDraftsParams, dict(requests=1, drafts=-1, vocab=5), -1, "bad shape"),
     ("grove_verify_drafts", _lib.VerifyDraftsParams, dict(requests=1, drafts=1, vocab=5), -1, "null"),
 ])
