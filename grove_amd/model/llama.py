@@ -254,6 +254,41 @@ class LlamaStack:
         # zero-filled: the graph-replayed step reads whole 64-key tiles and masks by kv_len; 0 * stale NaN would poison P V
         return [torch.zeros((B, 2, d.n_heads, S_max, d.head_dim), dtype=torch.bfloat16, device=self.dev) for _ in self.layers]
 
+    def new_kv4_cache(self, pages, page_size=64):
+        """The pages of a 4-bit cache that requests of unlike lengths share, one ops.KV4Cache per layer: 3.8 times the tokens of new_kv_cache in
+        the same memory at head_dim 128."""
+        d = self.d
+        return [ops.kv4_cache(pages, page_size, d.n_heads, d.head_dim, self.dev) for _ in self.layers]
+
+    def paged_step(self, x, step, table, cache, max_q, plan=None, max_len=None):
+        """One serving step over the paged 4-bit cache: x bf16 [rows, H] = the embeddings of every request's new tokens, packed (a prompt or a piece
+        of it, the next token, or that and drafted ones: ops.verify_drafts takes the logits' probabilities); step: the ops.PageStep that
+        ops.page_tables made for these rows with `table`; cache: new_kv4_cache; max_q: the most new tokens of a request; plan: ops.rotary_plan for
+        contexts longer than trained (default: the plain one); max_len: ops.kv4_attn's. Returns the final-norm hidden rows [rows, H] (bf16)."""
+        d = self.d
+        nh, hd, I = d.n_heads, d.head_dim, d.mlp
+        if plan is None:
+            plan = getattr(self, "_rotary_plan", None)
+            if plan is None:
+                plan = self._rotary_plan = ops.rotary_plan(hd, d.rope_theta, device=self.dev)
+        T = x.shape[0]
+        f32 = self.fp32_stream
+        res = ops.to_f32(x) if f32 else None
+        t = None  # fp32 stream: branch output not yet added to the stream (as in forward)
+        for L, kv in zip(self.layers, cache):
+            h = ops.rmsnorm(t, L["ln1"], d.rms_eps, res=res) if f32 else ops.rmsnorm(x, L["ln1"], d.rms_eps)
+            qkv = self._qkv(L, h).view(T, 3 * nh, hd)
+            ops.rotary(qkv[:, :2 * nh], step.pos, plan, out=qkv[:, :2 * nh])
+            ops.kv4_append(qkv[:, nh:2 * nh], qkv[:, 2 * nh:], kv, step.slots)
+            o = ops.kv4_attn(qkv[:, :nh], kv, table, step.kv_len, step.cu_q, max_q, hd ** -0.5, max_len=max_len)
+            if f32:
+                h2 = ops.rmsnorm(self._lin(L, "wo", o), L["ln2"], d.rms_eps, res=res)
+                t = self._lin(L, "wd", ops.swiglu(self._lin(L, "wgu", h2), I))
+            else:
+                x1 = self._lin(L, "wo", o, residual=x)
+                x = self._lin(L, "wd", ops.swiglu(self._lin(L, "wgu", ops.rmsnorm(x1, L["ln2"], d.rms_eps)), I), residual=x1)
+        return ops.rmsnorm(t, self.norm, d.rms_eps, res=res) if f32 else ops.rmsnorm(x, self.norm, d.rms_eps)
+
     def _decode_body(self, x, pos, kv_cache, lm_head=None):
         """The launches of one cached step: six per layer — RMSNorm folded into the q|k|v GEMV, RoPE + cache append + one-query
         attention over n_split blocks per head + the merge of their partial results, o_proj GEMV (+residual), RMSNorm folded into

@@ -781,3 +781,58 @@ def test_serving_on_another_stream(dev):
         torch.cuda.synchronize()
         assert torch.equal(a, out) and torch.equal(b, out)
         assert all(torch.equal(s, r) and torch.equal(t, r) for s, t, r in zip(va, vb, ref))
+
+
+# ----------------------------------------------------------------------------- the decoder stack over the paged cache
+@pytest.mark.parametrize("stream", [f32, bf16])
+def test_decoder_stack_over_pages(dev, stream):
+    """LlamaStack.paged_step: a prompt in one step, another in two pieces, then drafts, against the same stack with fp64 attention over the values
+    that the cache stands for. The two differ by bf16 roundings: some eight of a layer's values, 2^-9 of each at most in the root mean square, in two
+    layers, so 2^-9 sqrt(16) = 2^-7 of the hidden rows, doubled for what the norms and the residual sums pass on."""
+    from grove_amd import ops
+    from grove_amd.model.llama import LlamaStack
+    from grove_amd.synthetic import TINY, synthetic_state_dict
+    d = TINY
+    sd = {k: v.to(dev).to(bf16) for k, v in synthetic_state_dict(d).items() if k.startswith(("model.layers", "model.norm"))}
+    stack = LlamaStack(sd, d, dev, fp32_stream=stream == f32)
+    nh, hd, H, P = d.n_heads, d.head_dim, d.hidden, 16
+    cache = stack.new_kv4_cache(12, P)
+    table = torch.full((2, 5), -1, dtype=i32, device=dev)
+    free = torch.randperm(12, generator=gen(1)).to(i32).to(dev)
+    ctx, held = torch.zeros(2, dtype=i32, device=dev), torch.zeros(2, dtype=i32, device=dev)
+    plan = ops.rotary_plan(hd, d.rope_theta, device=dev)
+
+    def by_hand(x, step, new):
+        """The same with torch in fp64 between the matrix products; the cache holds this step's rows already."""
+        w = lambda t: t.double().cpu()  # noqa: E731
+        norm = lambda t, g: t * torch.rsqrt((t * t).mean(-1, keepdim=True) + d.rms_eps) * w(g)  # noqa: E731
+        x, pos = w(x), step.pos.cpu()
+        for L, kv in zip(stack.layers, cache):
+            qkv = (norm(x, L["ln1"]) @ w(L["wqkv"]).T).view(-1, 3 * nh, hd)
+            q = rotary_ref(qkv[:, :nh], pos, plan.freq.cpu(), False, 1.0)[0]
+            o, at = [], 0
+            for b, n in enumerate(new):
+                L_ = int(step.kv_len[b])
+                idx = torch.arange(L_, device=dev)
+                k, v = (t.cpu().double() for t in ops.kv4_read(kv, (table[b, idx // P] * P + idx % P).to(i32), f32))
+                z = torch.einsum("nhd,lhd->hnl", q[at:at + n], k) * hd ** -0.5
+                z = z.masked_fill(torch.arange(L_)[None] >= torch.arange(L_ - n + 1, L_ + 1)[:, None], -math.inf)
+                o.append(torch.einsum("hnl,lhd->nhd", torch.softmax(z, -1), v).flatten(1))
+                at += n
+            x = x + torch.cat(o) @ w(L["wo"]).T
+            g, u = (norm(x, L["ln2"]) @ w(L["wgu"]).T).split(d.mlp, -1)
+            x = x + (torch.nn.functional.silu(g) * u) @ w(L["wd"]).T
+        return norm(x, stack.norm)
+
+    for i, new in enumerate([[29, 10], [0, 21], [4, 4], [1, 1]]):
+        T = sum(new)
+        step = ops.page_tables(ctx, torch.tensor(new, dtype=i32, device=dev), table, held, free, P, T)
+        free, held = free[int(step.taken):], step.held
+        x = (torch.randn(T, H, generator=gen(20 + i)) * 0.5).to(bf16).to(dev)
+        out = stack.paged_step(x, step, table, cache, max(new)).double().cpu()
+        ref = by_hand(x, step, new)
+        err = ((out - ref).pow(2).mean() / ref.pow(2).mean()).sqrt().item()
+        assert err <= 2.0 ** -6, (i, err)
+        ctx = step.kv_len.clone()
+        if i == 2:
+            ctx = ctx - 2  # two drafts of each refused: their rows are written again
