@@ -1320,7 +1320,7 @@ def rotary(x, pos, plan, *, backward=False, out=None):
     _lens(what, "pos", pos, rows)
     if out is None:
         _need_device(what, x)
-        out = x.new_empty((rows, heads, hd))
+        out = torch.empty_like(x) if x.is_contiguous() else x.new_empty((rows, heads, hd))
         yr, yh = heads * hd, hd
     else:
         if out.shape != x.shape or out.dtype != dt or (out.stride(2) != 1 and hd > 1 and out.numel()):
@@ -1352,31 +1352,31 @@ def page_tables(ctx_len, new_len, table, held, free, page_size, rows):
     page numbers, used from the front; rows: the rows of the step, sum(new_len), or more for a step of fixed size. The caller drops the first
     `taken` of `free` (taken > len(free): the pages ran out, the rows without a page have slot -1)."""
     what = "page_tables"
-    if table.dim() != 2 or table.dtype != torch.int32 or 0 in table.shape or table.stride(1) != 1 or not _own_elements(table):
+    if table.dtype != _i32 or table.dim() != 2 or 0 in table.shape or table.stride(1) != 1 or not (table.is_contiguous() or _own_elements(table)):
         _refuse(what, "table must be int32 [requests, max_pages], its rows contiguous and apart")
     B, most = table.shape
-    _lens(what, "ctx_len", ctx_len, B)
-    _lens(what, "new_len", new_len, B)
-    _lens(what, "held", held, B)
-    _lens(what, "free", free, free.numel())
+    n_free = free.numel()
+    each, t0, ld = (B,), table.data_ptr(), most if B == 1 else table.stride(0)
+    t1 = t0 + 4 * ((B - 1) * ld + most)
+    at = []
+    for name, t, n in (("ctx_len", ctx_len, B), ("new_len", new_len, B), ("held", held, B), ("free", free, n_free)):
+        if t.dtype != _i32 or t.shape != (each if n == B else (n,)) or not t.is_contiguous():
+            _lens(what, name, t, n)
+        a = t.data_ptr()
+        if a < t1 and a + 4 * n > t0:
+            _refuse(what, "table overlaps an input")
+        at.append(a)
     if B > 4096:
         _refuse(what, f"{B} requests: at most 4096")
     if page_size < 1 or page_size & (page_size - 1):
         _refuse(what, "the page size must be a power of two")
     if not 0 <= rows < 2 ** 31:
         _refuse(what, "bad number of rows")
-    ld = max(table.stride(0), most)
-    t0 = table.data_ptr()
-    t1 = t0 + 4 * ((B - 1) * ld + most)
-    at = [t.data_ptr() for t in (ctx_len, new_len, held, free)]
-    for a, n in zip(at, (B, B, B, free.shape[0])):
-        if a < t1 and a + 4 * n > t0:
-            _refuse(what, "table overlaps an input")
     _need_device(what, table)
     o = table.new_empty(3 * B + 2 + 2 * rows)  # one allocation for the six results
     o0 = o.data_ptr()
     o1, o2, o3, o4, o5 = o0 + 4 * B, o0 + 8 * B + 4, o0 + 8 * B + 4 + 4 * rows, o0 + 8 * B + 4 + 8 * rows, o0 + 12 * B + 4 + 8 * rows
-    p = _pack_pagetables(*at, t0, o0, o1, o2, o3, o4, o5, ld, B, most, page_size, rows, free.shape[0])
+    p = _pack_pagetables(*at, t0, o0, o1, o2, o3, o4, o5, ld, B, most, page_size, rows, n_free)
     _launch(what, p, table, ctx_len, new_len, held, free)
     return PageStep(*o.split_with_sizes((B, B + 1, rows, rows, B, 1)))
 
