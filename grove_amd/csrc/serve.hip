@@ -316,9 +316,11 @@ struct draw_lds {
 };
 // Of 4 x 256 weights, 4 consecutive ones a thread: the first whose running sum (from `carry`) passes thr, else the last that is not 0, else -1; by
 // ballots (atomics on one LDS word take their lanes one after the other). `sum`: of all; s.before, after a barrier: the sum before the one found.
-__device__ int search(const double (&r)[4], double carry, double thr, draw_lds& s, double& sum, bool& passed) {
+// pick >= 0: thr becomes that part of the sum first.
+__device__ int search(const double (&r)[4], double carry, float pick, double& thr, draw_lds& s, double& sum, bool& passed) {
   const int tid = threadIdx.x, w = tid >> 6;
   const double own = (r[0] + r[1]) + (r[2] + r[3]), before = carry + (block_scan(own, s.wsum, sum) - own);
+  if (pick >= 0.f) thr = (double)pick * sum;
   int low = 4, last = -1;
   double c[5];
   c[0] = before;
@@ -354,21 +356,19 @@ template <typename T>
 __device__ int draw(const rest_row<T>& row, int V, float pick, draw_lds& s) {
   const int tid = threadIdx.x, chunk = vd_chunk(V), nchunk = vd_chunks(V);
   __syncthreads();  // the sums are there
-  double r[4], total = 0, part;
+  double r[4], total, part, thr = 0;
   bool passed;
 #pragma unroll
   for (int i = 0; i < 4; ++i) r[i] = 4 * tid + i < nchunk ? s.sums[4 * tid + i] : 0.0;
-  block_scan((r[0] + r[1]) + (r[2] + r[3]), s.wsum, total);
-  if (!(total > 0)) return -1;
-  const double thr = (double)pick * total;
-  const int c = search(r, 0.0, thr, s, part, passed);
+  const int c = search(r, 0.0, pick, thr, s, total, passed);
+  if (c < 0) return -1;
   __syncthreads();
   double carry = s.before;
   int last = -1;
   for (int j0 = c * chunk; j0 < min(V, (c + 1) * chunk); j0 += 1024) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) r[i] = j0 + 4 * tid + i < V ? row.one(j0 + 4 * tid + i) : 0.0;
-    const int at = search(r, carry, thr, s, part, passed);
+    const int at = search(r, carry, -1.f, thr, s, part, passed);
     if (at >= 0) last = j0 + at;
     if (passed) return last;
     carry += part;
