@@ -86,6 +86,7 @@ __global__ __launch_bounds__(256) void norm_fwd_kernel(const grove_norm_params p
     if (lane + i * 64 < nch) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
+#pragma clang fp contract(off)  // (squares rounded, then added: the statistics do not depend on what the compiler makes of the loop)
         const float d = r.v[i][e] - mean;
         ss += d * d;
       }
