@@ -308,6 +308,17 @@ __global__ __launch_bounds__(256, kv4_waves(HD, CT)) void kv4_attn_kernel(const 
   }
   const int t0 = max(0, min(q_lo, p.rows)), t1 = max(t0, min(q_hi, p.rows)), n = t1 - t0;
   const int cols = min(n, p.max_q) * G, col0 = cc * 16 * CT;
+  if (n > p.max_q && cc == chunks - 1) {  // more new tokens than the call allows for: NaN, not what the memory held
+    for (int e = tid; e < (n - p.max_q) * G; e += 256) {
+      const int64_t row = t0 + p.max_q + e / G, head = hk * G + e % G;
+      if (p.n_split > 1) {
+        float* ml = p.partial + (int64_t)p.rows * p.heads * p.n_split * HD + ((row * p.heads + head) * p.n_split + sp) * 2;
+        ml[0] = 0.f;
+        ml[1] = NAN;
+      } else
+        for (int c = 0; c < HD / 2; ++c) ((unsigned*)((bf16_raw*)p.out + row * p.so_row + head * HD))[c] = 0x7fc07fc0u;
+    }
+  }
   if (col0 >= cols) return;
   const int64_t room = (int64_t)p.max_pages << shift;
   const int base = (int)min((int64_t)max(kv_len, 0), room) - n + 1;  // token i sees base + i keys
@@ -413,9 +424,12 @@ __global__ __launch_bounds__(256, kv4_waves(HD, CT)) void kv4_attn_kernel(const 
 
   // A wave's tiles. A column's reference is the maximum of its first keys; the accumulators are never rescaled: where a later score passes it by 24
   // (P <= 2^24 loses nothing in fp32) the wave starts again with that score's reference. Scores that far above a wave's first 32 keys' are rare, and
-  // rescaling in the loop costs a second set of registers for the accumulators (57 of them at CT = 2) or a copy of each per tile.
+  // rescaling in the loop costs a second set of registers for the accumulators (57 of them at CT = 2) or a copy of each per tile. The second start
+  // reads the keys alone, for the references that hold to the end: scores that climb along the context cost three passes, not one per climb (8
+  // requests of 8192 keys that climb by 0.32 a key: 73 us -> 38, with 5 tokens each 218 -> 59, against 23 and 36 without a climb; the test costs 1 %).
   f32x4_t acc[CT][NJ];
   int tile, from;
+  bool keys_only = false;
   float z[CT][8], top[CT];
   auto raise = [&]() -> bool {  // new references for the columns whose scores passed theirs; true: something was summed with an old one
     bool again = false;
@@ -508,9 +522,14 @@ __global__ __launch_bounds__(256, kv4_waves(HD, CT)) void kv4_attn_kernel(const 
       }
       if (__any(grow)) {
         if constexpr (HD * CT >= 512) return 2;  // (outside of the loop: inside it the paths' joined registers do not fit)
-        if (raise()) return 1;
+        if (raise() && !keys_only) return 1;
       }
       if (ahead < tile1) issue();
+      if (keys_only) {
+        tile += 4;
+        from = from == S - 1 ? 0 : from + 1;
+        continue;
+      }
       ring_read<HD, 2 * PART, 4 * PART + 128>(at_values, at_scales, T.v, T.vs);
       if (masked) {  // 0 times a scale that is no number would reach the columns that do not see its row: it goes, and those that see it become NaN
         unsigned odd = 0;
@@ -593,7 +612,7 @@ __global__ __launch_bounds__(256, kv4_waves(HD, CT)) void kv4_attn_kernel(const 
   ask_q();
   fill();
   use_q();
-  while (true) {
+  for (int starts = 0;; ++starts) {
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
       l[ct] = cst[ct] = 0.f;
@@ -601,9 +620,10 @@ __global__ __launch_bounds__(256, kv4_waves(HD, CT)) void kv4_attn_kernel(const 
       for (int j = 0; j < NJ; ++j) acc[ct][j] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
     }
     int left;
-    while ((left = run()) == 2 && !raise()) {
+    keys_only = starts == 2;
+    while ((left = run()) == 2 && (!raise() || keys_only)) {
     }
-    if (left == 0) break;
+    if (left == 0 && !keys_only) break;
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the tiles in flight land before their slots are asked for again
     start();
     fill();
@@ -756,7 +776,7 @@ bool hd_ok(int hd) { return hd == 32 || hd == 64 || hd == 128 || hd == 256; }
   }
 
 extern "C" int grove_kv4_append(const grove_kv4_append_params* p, void* stream) {
-  GROVE_CHECK(p && p->rows >= 0 && p->kv > 0 && p->kv <= 65535, GROVE_E_SHAPE, "kv4_append: bad shape");
+  GROVE_CHECK(p && p->rows >= 0 && p->rows <= 1 << 30 && p->kv > 0 && p->kv <= 65535, GROVE_E_SHAPE, "kv4_append: bad shape");
   KV4_SHAPE(p, "kv4_append");
   if (p->rows == 0) return GROVE_OK;
   GROVE_CHECK(p->k && p->v && p->codes && p->scales && p->slots, GROVE_E_SHAPE, "kv4_append: null pointer");
@@ -772,7 +792,7 @@ extern "C" int grove_kv4_append(const grove_kv4_append_params* p, void* stream) 
 }
 
 extern "C" int grove_kv4_read(const grove_kv4_read_params* p, void* stream) {
-  GROVE_CHECK(p && p->rows >= 0 && p->kv > 0 && p->kv <= 65535, GROVE_E_SHAPE, "kv4_read: bad shape");
+  GROVE_CHECK(p && p->rows >= 0 && p->rows <= 1 << 30 && p->kv > 0 && p->kv <= 65535, GROVE_E_SHAPE, "kv4_read: bad shape");
   KV4_SHAPE(p, "kv4_read");
   if (p->rows == 0) return GROVE_OK;
   GROVE_CHECK(p->k && p->v && p->codes && p->scales && p->slots, GROVE_E_SHAPE, "kv4_read: null pointer");
@@ -804,7 +824,8 @@ extern "C" int grove_kv4_attn(const grove_kv4_attn_params* p, void* stream) {
   // columns that one pass over a key can serve: as few tiles of 16 as hold them, at most 64 (32 at hd 256, whose outputs fill the registers)
   const int64_t cols = (int64_t)(p->max_q < p->rows ? p->max_q : p->rows) * (p->heads / p->kv);
   const int ct = cols <= 16 ? 1 : cols <= 32 || p->hd == 256 ? 2 : 4;
-  const int64_t chunks = (cols + 16 * ct - 1) / (16 * ct);
+  const int64_t chunks = (cols + 16 * ct - 1) / (16 * ct), units = (int64_t)p->rows * p->heads;
+  GROVE_CHECK(units <= 1 << 30 && (p->n_split <= 8 || units < 1 << 24), GROVE_E_SHAPE, "kv4_attn: too many rows");
   GROVE_CHECK(chunks * p->kv <= 65535, GROVE_E_SHAPE, "kv4_attn: too many new tokens in a request (%lld columns)", (long long)cols);
   const dim3 grid((unsigned)p->n_split, (unsigned)(chunks * p->kv), (unsigned)p->requests);
 #define RUN(HD, CT)                                                                                                                  \
@@ -822,8 +843,6 @@ extern "C" int grove_kv4_attn(const grove_kv4_attn_params* p, void* stream) {
 #undef RUN
   GROVE_LAUNCH_CHECK();
   if (p->n_split > 1) {
-    const int64_t units = (int64_t)p->rows * p->heads;
-    GROVE_CHECK(units <= 0x7fffffff, GROVE_E_SHAPE, "kv4_attn: too many rows");
 #define LAUNCH(HD)                                                                                                                                  \
   if (p->n_split > 8) hipLaunchKernelGGL((kv4_join_kernel<HD, 4>), dim3((unsigned)units), dim3(256), 0, (hipStream_t)stream, *p);                   \
   else hipLaunchKernelGGL((kv4_join_kernel<HD, 1>), dim3((unsigned)((units + 3) / 4)), dim3(256), 0, (hipStream_t)stream, *p)

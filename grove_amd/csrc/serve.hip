@@ -428,7 +428,7 @@ __global__ __launch_bounds__(256) void verify_sums_kernel(const grove_verify_dra
 }  // namespace
 
 extern "C" int grove_rotary(const grove_rotary_params* p, void* stream) {
-  GROVE_CHECK(p && p->rows >= 0 && p->heads >= 0 && p->hd > 0 && p->rot >= 0 && p->rot <= p->hd && (p->rot & 1) == 0 && (int64_t)p->heads * p->hd < (1 << 28),
+  GROVE_CHECK(p && p->rows >= 0 && p->rows <= 1 << 30 && p->heads >= 0 && p->hd > 0 && p->rot >= 0 && p->rot <= p->hd && (p->rot & 1) == 0 && (int64_t)p->heads * p->hd < (1 << 28),
               GROVE_E_SHAPE, "rotary: bad shape");
   if (p->rows == 0 || p->heads == 0) return GROVE_OK;
   GROVE_CHECK(p->x && p->y && p->pos && (p->freq || p->rot == 0), GROVE_E_SHAPE, "rotary: null pointer");

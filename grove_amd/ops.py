@@ -1290,8 +1290,8 @@ def rotary_plan(rot, theta=10000.0, *, interleaved=False, scaling="none", factor
     if scaling == "linear":
         w = w / factor
     elif scaling == "yarn":
-        if not (trained_len > 0 and fast > slow > 0):
-            _refuse(what, "yarn needs trained_len > 0 and fast > slow > 0")
+        if not (fast > slow > 0 and trained_len > 2 * math.pi * slow):
+            _refuse(what, "yarn needs fast > slow > 0 and a trained_len in which the first pair turns more than slow times")
 
         def pair(turns):  # the (real) number of the pair that turns so many times in trained_len
             return rot * math.log(trained_len / (turns * 2 * math.pi)) / (2 * math.log(theta))
@@ -1467,7 +1467,7 @@ def _kv4_split(pairs, max_len, cols, hd):
 def kv4_attn(q, cache, table, kv_len, cu_q, max_q, alpha, *, max_len=None, out=None):
     """Causal attention of every request's new tokens over its 4-bit pages (grove_kv4_attn). q: bf16 [rows, heads, hd], any row and head strides
     (read in place where they are multiples of 8 from a 16-byte aligned start); table int32 [requests, max_pages]; kv_len int32 [requests] keys including the new tokens; cu_q int32 [requests + 1] (page_tables makes both);
-    max_q: the most new tokens that any request has. max_len: the longest kv_len if the host knows it (default: what the table holds); only the
+    max_q: the most new tokens that any request has (rows past it become NaN). max_len: the longest kv_len if the host knows it (default: what the table holds); only the
     split of the work goes by it. Returns bf16 [rows, heads * hd]; rows of no request are zero in a new tensor and stay as they were in `out`."""
     what = "kv4_attn"
     pages, kv, P, hd = _kv4_shape(what, cache)

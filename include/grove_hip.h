@@ -710,7 +710,9 @@ int grove_kv4_read(const grove_kv4_read_params* p, void* stream);
  *   row r = cu_q[b] + i of request b with n = cu_q[b + 1] - cu_q[b] new tokens sees the keys t < kv_len[b] - n + i + 1:
  *   out[r] = softmax(alpha * q[r] . K[t]) V, fp32 throughout; 0 where it sees none.
  * Keys whose table entry is outside [0, pages) are not seen. kv_len is cut to max_pages * page. Rows of no request are left as they
- * were. n must not pass max_q, a row of the table not 2^30 tokens. q and its strides are aligned to 16 bytes, out and its row stride to 4. Rows of the cache that no query sees may hold anything.
+ * were; so are all with requests or max_q 0. n does not pass max_q (a request's rows past it become NaN), a row of the table not 2^30 tokens,
+ * rows * heads not 2^30, nor 2^24 with more than 8 splits. q and its strides are aligned to 16 bytes, out and its row stride to 4. Rows of the
+ * cache that no query sees may hold anything.
  * n_split > 1 (at most 64): a request's keys are dealt to n_split blocks, whose partial results lie in `partial`, f32 [rows * heads * n_split *
  * (hd + 2)], and are joined by a second launch. Otherwise `partial` may be NULL. */
 typedef struct grove_kv4_attn_params {

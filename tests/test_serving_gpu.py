@@ -431,6 +431,48 @@ def test_attn_climbing_scores(dev, H, kv, new, hd):
     within(out, ref, tol)
 
 
+@pytest.mark.parametrize("H,kv,new,hd", [(4, 4, 1, 32), (2, 1, 1, 64), (8, 2, 2, 128), (8, 1, 4, 128), (8, 1, 8, 128), (16, 1, 4, 64), (4, 4, 1, 256), (8, 2, 5, 256)])
+@pytest.mark.parametrize("max_len", [1, None])
+def test_attn_scores_that_climb_all_along(dev, H, kv, new, hd, max_len):
+    """Every 128 keys pass the references of those before them (by some 40 in units of log2), one and many blocks per pair."""
+    from grove_amd import ops
+    L, P = 3000, 64
+    c = Paged(dev, [L, 40], kv, hd, P, seed=73)
+    g = gen(74)
+    q = (1.0 + 0.1 * torch.randn(new + 1, H, hd, generator=g)).to(bf16)
+    k = (torch.arange(L) * 0.22 / hd)[:, None, None] * (1 + 0.1 * torch.rand(1, kv, hd, generator=g))
+    v = torch.randn(L, kv, hd, generator=g)
+    ops.kv4_append(k.to(bf16).to(dev), v.to(bf16).to(dev), c.cache, c.slots[:L])
+    kk, vv = (t.cpu().to(f64) for t in ops.kv4_read(c.cache, c.slots, f32))
+    c.k, c.v = kk.split([L, 40]), vv.split([L, 40])
+    step = [(t.amax(-1) - t.amin(-1)) / 15 for t in (kk, vv)]
+    c.size = [float(31 * s.max() + t.abs().max()) for s, t in zip(step, (kk, vv))]
+    cu = torch.tensor([0, new, new + 1], dtype=i32, device=dev)
+    out = ops.kv4_attn(q.to(dev), c.cache, c.table, torch.tensor([L, 40], dtype=i32, device=dev), cu, new, 1.0, max_len=max_len)
+    ref, tol = c.ref(q, [new, 1], 1.0)
+    within(out, ref, tol)
+
+
+@pytest.mark.parametrize("max_len", [1, 4000])
+@pytest.mark.parametrize("H,kv,hd", [(4, 2, 64), (24, 2, 128)])
+def test_attn_more_new_tokens_than_said(dev, H, kv, hd, max_len):
+    """Rows past max_q are NaN, whatever the memory held, and the others right."""
+    from grove_amd import ops
+    c = Paged(dev, [300, 50, 7], kv, hd, 16, seed=75)
+    new = [4, 2, 3]
+    q = torch.randn(10, H, hd, generator=gen(76)).to(bf16)
+    cu = torch.tensor([0, 4, 6, 9], dtype=i32, device=dev)
+    kv_len = torch.tensor(c.lens, dtype=i32, device=dev)
+    ref, tol = c.ref(q[:9], new, 0.1)
+    for given in (False, True):
+        out = torch.full((10, H * hd), 5.0, dtype=bf16, device=dev) if given else None
+        got = ops.kv4_attn(q.to(dev), c.cache, c.table, kv_len, cu, 2, 0.1, max_len=max_len, out=out).cpu()
+        past = torch.tensor([0, 0, 1, 1, 0, 0, 0, 0, 1, 0], dtype=torch.bool)
+        assert got[past].isnan().all()
+        within(got[:9][~past[:9]], ref[~past[:9]], tol[~past[:9]])
+        assert (got[9] == (5.0 if given else 0.0)).all()
+
+
 def test_attn_single_key_is_its_value(dev):
     c, q, cu, kv_len, out = check_attn(dev, [1, 1], [1, 1], 4, 2, 128, 16)
     v = torch.stack([c.v[b][0].repeat_interleave(2, 0) for b in range(2)]).flatten(1)
