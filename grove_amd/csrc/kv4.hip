@@ -252,7 +252,7 @@ __device__ __forceinline__ void ring_read(unsigned a, unsigned as, unsigned (&w)
       asm volatile("ds_read_b128 %0, %6 offset:%8\n\tds_read_b128 %1, %6 offset:%9\n\tds_read_b128 %2, %6 offset:%10\n\tds_read_b128 %3, %6 offset:%11\n\t"
                    "ds_read_b128 %4, %7 offset:%12\n\tds_read_b128 %5, %7 offset:%13\n\ts_waitcnt lgkmcnt(0)"
                    : "=&v"(x[0][0]), "=&v"(x[0][N - 1]), "=&v"(x[1][0]), "=&v"(x[1][N - 1]), "=&v"(s[0]), "=&v"(s[1])
-                   : "v"(a), "v"(as), "n"(O), "n"(O + 1024), "n"(O + 2048), "n"(O + 3072), "n"(OS), "n"(OS + 64) : "memory");
+                   : "v"(a), "v"(as), "n"(O), "n"(O + 1024), "n"(O + 2 * 1024), "n"(O + 3 * 1024), "n"(OS), "n"(OS + 64) : "memory");
     }
 #pragma unroll
     for (int u = 0; u < 2; ++u)
@@ -371,7 +371,7 @@ __global__ __launch_bounds__(256, kv4_waves(HD, CT)) void kv4_attn_kernel(const 
     asm volatile("ds_read_b128 %0, %5 offset:%7\n\tds_read_b128 %1, %5 offset:%8\n\tds_read_b128 %2, %5 offset:%9\n\tds_read_b128 %3, %5 offset:%10\n\t"
                  "ds_read_b32 %4, %6\n\ts_waitcnt lgkmcnt(0)"
                  : "=&v"(f[0]), "=&v"(f[1 % NK]), "=&v"(f[2 % NK]), "=&v"(f[3 % NK]), "=&v"(sum)
-                 : "v"(at), "v"(qs_at + ct * 64), "n"(0), "n"(1024), "n"(2048), "n"(3072) : "memory");
+                 : "v"(at), "v"(qs_at + ct * 64), "n"(0), "n"(1024), "n"(2 * 1024), "n"(3 * 1024) : "memory");
   };
   // page numbers by scalar loads (the constant address space), asked for one tile ahead of their use
   const scalar_ints row = (scalar_ints)(uintptr_t)(p.table + b * p.ld_table);
