@@ -811,7 +811,7 @@ extern "C" int grove_kv4_read(const grove_kv4_read_params* p, void* stream) {
 
 extern "C" int grove_kv4_attn(const grove_kv4_attn_params* p, void* stream) {
   GROVE_CHECK(p && p->requests >= 0 && p->requests <= 65535 && p->rows >= 0 && p->kv > 0 && p->heads > 0 && p->heads % p->kv == 0 && p->heads <= 65535 &&
-              p->max_pages > 0 && p->ld_table >= p->max_pages && p->max_q >= 0, GROVE_E_SHAPE, "kv4_attn: bad shape (heads must be a multiple of kv)");
+              p->max_pages > 0 && p->ld_table >= 0 && p->max_q >= 0, GROVE_E_SHAPE, "kv4_attn: bad shape (heads must be a multiple of kv)");
   KV4_SHAPE(p, "kv4_attn");
   if (p->rows == 0 || p->requests == 0 || p->max_q == 0) return GROVE_OK;
   GROVE_CHECK(p->q && p->codes && p->scales && p->table && p->kv_len && p->cu_q && p->out, GROVE_E_SHAPE, "kv4_attn: null pointer");

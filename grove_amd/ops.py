@@ -1466,7 +1466,8 @@ def _kv4_split(pairs, max_len, cols, hd):
 
 def kv4_attn(q, cache, table, kv_len, cu_q, max_q, alpha, *, max_len=None, out=None):
     """Causal attention of every request's new tokens over its 4-bit pages (grove_kv4_attn). q: bf16 [rows, heads, hd], any row and head strides
-    (read in place where they are multiples of 8 from a 16-byte aligned start); table int32 [requests, max_pages]; kv_len int32 [requests] keys including the new tokens; cu_q int32 [requests + 1] (page_tables makes both);
+    (read in place where they are multiples of 8 from a 16-byte aligned start); table int32 [requests, max_pages], its rows
+    contiguous (requests may share one: an expanded row); kv_len int32 [requests] keys including the new tokens; cu_q int32 [requests + 1] (page_tables makes both);
     max_q: the most new tokens that any request has (rows past it become NaN). max_len: the longest kv_len if the host knows it (default: what the table holds); only the
     split of the work goes by it. Returns bf16 [rows, heads * hd]; rows of no request are zero in a new tensor and stay as they were in `out`."""
     what = "kv4_attn"
@@ -1509,7 +1510,7 @@ def kv4_attn(q, cache, table, kv_len, cu_q, max_q, alpha, *, max_len=None, out=N
     # the joined splits' workspace: from the allocator at every call, so that calls on other streams and captured graphs have their own
     partial = q.new_empty(rows * heads * n_split * (hd + 2), dtype=_f32) if n_split > 1 else None
     p = _pack_kv4attn(q.data_ptr(), codes.data_ptr(), scales.data_ptr(), table.data_ptr(), kv_len.data_ptr(), cu_q.data_ptr(), out.data_ptr(),
-                           0 if partial is None else partial.data_ptr(), qr, qh, orow, max(table.stride(0), most), B, heads, kv, hd, P, pages, most,
+                           0 if partial is None else partial.data_ptr(), qr, qh, orow, most if B == 1 else table.stride(0), B, heads, kv, hd, P, pages, most,
                            rows, max_q, n_split, fresh, alpha)
     _launch(what, p, q, codes, scales, table, kv_len, cu_q, out)
     return out

@@ -719,7 +719,7 @@ typedef struct grove_kv4_attn_params {
   const void* q;
   const void* codes;
   const void* scales;
-  const int32_t* table;  /* [requests, ld_table] */
+  const int32_t* table;  /* [requests, ld_table]; only read: rows may overlap, ld_table 0 is one row for all */
   const int32_t* kv_len; /* [requests] */
   const int32_t* cu_q;   /* [requests + 1] */
   void* out;

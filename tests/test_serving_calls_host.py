@@ -1,0 +1,57 @@
+"""What the serving operators hand to their C entries, with the launch replaced: no GPU needed."""
+import ctypes
+
+import pytest
+import torch
+
+from grove_amd import _lib, ops
+
+bf16, i32 = torch.bfloat16, torch.int32
+
+
+def ints(*v):
+    return torch.tensor(v, dtype=i32)
+
+
+@pytest.fixture
+def launched(monkeypatch):
+    """The params and tensors of every launch, in order, as (name, params struct, tensors)."""
+    calls = []
+    structs = {"kv4_attn": _lib.Kv4AttnParams}
+
+    def launch(name, params, *ts):
+        calls.append((name, structs[name].from_buffer_copy(params), ts))
+    monkeypatch.setattr(ops, "_launch", launch)
+    monkeypatch.setattr(ops, "_need_device", lambda what, t: None)
+    return calls
+
+
+def attn(q, table, out=None, rows_of=(1, 1, 1)):
+    c = ops.kv4_cache(4, 16, 2, 64, "cpu")
+    B = table.shape[0]
+    cu = ints(0, *torch.tensor(rows_of).cumsum(0).tolist())
+    return ops.kv4_attn(q, c, table, torch.full((B,), 9, dtype=i32), cu, max(rows_of), 1.0, out=out)
+
+
+# ----------------------------------------------------------------------------- tables
+@pytest.mark.parametrize("make,stride", [
+    (lambda t: t[:1].expand(3, 5), 0),                       # one page list for requests that share a context
+    (lambda t: t.view(-1).as_strided((3, 5), (2, 1)), 2),    # rows that overlap: the kernel only reads them
+    (lambda t: t, 5),
+    (lambda t: torch.zeros(3, 9, dtype=i32)[:, :5], 9)])
+def test_attn_table_rows_keep_their_stride(launched, make, stride):
+    """No request's row is looked for behind the tensor."""
+    table = make(torch.arange(15, dtype=i32).view(3, 5))
+    attn(torch.zeros(3, 4, 64, dtype=bf16), table)
+    (_, p, _), = launched
+    assert p.ld_table == stride and p.max_pages == 5
+    last = p.table + 4 * (2 * p.ld_table + p.max_pages)
+    assert last <= table.untyped_storage().data_ptr() + table.untyped_storage().nbytes()
+
+
+def test_attn_entry_takes_shared_table_rows():
+    """ld_table below max_pages passes the shape check (the next one, null pointers, refuses); a negative one does not."""
+    fields = dict(requests=2, rows=1, heads=2, kv=2, hd=64, page=16, pages=1, max_pages=4, max_q=1)
+    for ld, text in ((0, "null"), (1, "null"), (-4, "bad shape")):
+        p = _lib.Kv4AttnParams(**fields, ld_table=ld)
+        assert _lib.lib().grove_kv4_attn(ctypes.byref(p), None) == -1 and text in _lib.last_error(), ld
