@@ -531,12 +531,12 @@ __global__ __launch_bounds__(256, kv4_waves(HD, CT)) void kv4_attn_kernel(const 
         continue;
       }
       ring_read<HD, 2 * PART, 4 * PART + 128>(at_values, at_scales, T.v, T.vs);
-      if (masked) {  // 0 times a scale that is no number would reach the columns that do not see its row: it goes, and those that see it become NaN
+      if (masked) {  // 0 times a minimum that is no number would reach the columns that do not see its row: it goes, and those that see it become NaN
         unsigned odd = 0;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           const unsigned sm = T.vs[i >> 2][i & 3];
-          const bool is = ((sm & 0x7f80u) == 0x7f80u) | ((sm & 0x7f800000u) == 0x7f800000u);
+          const bool is = !(fabsf(fmaf(-16.f, bf_lo(sm), bf_hi(sm))) < INFINITY);  // (what is used below: a finite scale of 2^124 overflows it)
           odd |= is ? 1u << i : 0u;
           T.vs[i >> 2][i & 3] = is ? 0u : sm;
         }

@@ -23,3 +23,76 @@ def test_attn_shared_table_row(dev, max_len):
     for table in (c.table.expand(3, -1), wide.as_strided((3, c.table.shape[1]), (2, 1))):
         a, b = (ops.kv4_attn(q, c.cache, t, kv_len, cu, 4, 0.125, max_len=max_len) for t in (table, table.contiguous()))
         assert torch.equal(a, b) and a.isfinite().all() and not (a == 0).all(1).any()
+
+
+# ----------------------------------------------------------------------------- what rows may hold
+SHAPES = [(4, 4, 1, 32), (4, 2, 4, 64), (2, 2, 1, 128), (8, 1, 4, 128), (16, 1, 4, 128), (4, 4, 1, 256), (8, 1, 4, 256), (16, 1, 4, 64)]  # every form of the kernel
+POISON = [0x7f00, 0xff00, 0x7d80, 0x7f7f, 0xfd81, 0x7f80, 0x7fc0, 0x8001]  # scales and minima: finite ones from 2^124, infinity, NaN, a denormal
+
+
+def poisoned(c, bits_s, bits_m):
+    """Every cache row of `c` that no request owns holds (bits_s, bits_m) as its scale and minimum."""
+    word = torch.tensor([bits_s, bits_m], dtype=i32).to(torch.int16).to(c.dev)
+    flat = c.cache.scales.view(torch.int16)
+    keep = torch.zeros(flat.shape[0] * c.P, dtype=torch.bool, device=c.dev)
+    keep[c.slots.long()] = True
+    keep = keep.view(-1, 1, 1, c.P, 1).expand_as(flat)
+    flat.copy_(torch.where(keep, flat, word.expand_as(flat)))
+
+
+@pytest.mark.parametrize("max_len", [1, 100000])
+@pytest.mark.parametrize("H,kv,new,hd", SHAPES)
+def test_attn_unseen_rows_hold_any_bits(dev, H, kv, new, hd, max_len):
+    """Rows behind the lengths and those of other pages (page 0 stands in for a page outside the cache), whatever finite or other numbers they hold."""
+    from grove_amd import ops
+    lens, P, alpha = [45, 83, 16 + new], 16, hd ** -0.5
+    c, q, cu, kv_len, _ = check_attn(dev, lens, [new] * 3, H, kv, hd, P, seed=hd + H, max_len=max_len)
+    table = c.table.clone()
+    table[1, 1] = -1  # its keys drop out
+    qd = q.to(dev)
+    first = [ops.kv4_attn(qd, c.cache, t, kv_len, cu, new, alpha, max_len=max_len) for t in (c.table, table)]
+    assert first[0].isfinite().all() and first[1].isfinite().all()
+    for s in POISON:
+        for m in (POISON[0], POISON[1], 0x3f80):
+            poisoned(c, s, m)
+            for t, ref in zip((c.table, table), first):
+                assert torch.equal(ops.kv4_attn(qd, c.cache, t, kv_len, cu, new, alpha, max_len=max_len), ref), (hex(s), hex(m))
+
+
+@pytest.mark.parametrize("H,kv,new,hd", [s for s in SHAPES if s[2] > 1])
+def test_attn_a_huge_row_stays_with_those_who_see_it(dev, H, kv, new, hd):
+    """The last token's value row with a range just below the end of fp32 (scale 2^124): the last query of the request is no number or infinite, the
+    others and the other request as they were."""
+    from grove_amd import ops
+    lens, P, alpha = [45, 80], 16, hd ** -0.5
+    c, q, cu, kv_len, out = check_attn(dev, lens, [new] * 2, H, kv, hd, P, seed=hd + H + 3)
+    k, v = (torch.zeros(1, kv, hd) for _ in range(2))
+    v[0, 0, 1], v[0, 0, 2] = 1.65e38, -1.65e38
+    ops.kv4_append(k.to(bf16).to(dev), v.to(bf16).to(dev), c.cache, c.slots[44:45])
+    assert ops.kv4_read(c.cache, c.slots[44:45], f32)[1].isfinite().all()
+    r = ops.kv4_attn(q.to(dev), c.cache, c.table, kv_len, cu, new, alpha)
+    keep = torch.ones(2 * new, dtype=torch.bool)
+    keep[new - 1] = False
+    assert torch.equal(r[keep], out[keep]) and not r[new - 1].view(H, hd)[:H // kv].isfinite().any()
+
+
+@pytest.mark.parametrize("max_len", [1, 100000])
+@pytest.mark.parametrize("H,kv,new,hd", SHAPES)
+def test_attn_values_to_two_to_the_64(dev, H, kv, new, hd, max_len):
+    """The largest values that are promised: powers of two pass through every sum exactly, keys' and queries' against each other too, also where the
+    weights are as large as they get (scores that climb by 23 in units of log2 behind a wave's first keys)."""
+    from grove_amd import ops
+    L, P = 1500, 32
+    c = Paged(dev, [L, 40], kv, hd, P, seed=7)
+    g = gen(8)
+    q = (1.0 + 0.1 * torch.randn(2 * new, H, hd, generator=g)).to(bf16)
+    k = torch.where(torch.arange(L) < 128, 0.0, 15.0)[:, None, None] / hd * (1 + 0.05 * torch.rand(L, kv, hd, generator=g))
+    v = torch.randn(L, kv, hd, generator=g).clamp(-1, 1)
+    cu = torch.tensor([0, new, 2 * new], dtype=i32, device=dev)
+    kv_len = torch.tensor([L, 40], dtype=i32, device=dev)
+    res = []
+    for ks, vs in ((1.0, 1.0), (2.0 ** 40, 2.0 ** 64), (2.0 ** -40, 2.0 ** -60)):
+        ops.kv4_append((k * ks).to(bf16).to(dev), (v * vs).to(bf16).to(dev), c.cache, c.slots[:L])
+        o = ops.kv4_attn((q / ks).to(bf16).to(dev), c.cache, c.table, kv_len, cu, new, 1.0, max_len=max_len)
+        res.append(o[:new].double() / vs)
+    assert res[0].isfinite().all() and torch.equal(res[0], res[1]) and torch.equal(res[0], res[2])
