@@ -321,7 +321,7 @@ __global__ __launch_bounds__(256, kv4_waves(HD, CT)) void kv4_attn_kernel(const 
   }
   if (col0 >= cols) return;
   const int64_t room = (int64_t)p.max_pages << shift;
-  const int base = (int)min((int64_t)max(kv_len, 0), room) - n + 1;  // token i sees base + i keys
+  const int base = (int)min((int64_t)max(kv_len, 0), room) - (q_hi - t0) + 1;  // token i sees base + i keys (of all its new tokens, also those past `rows`)
   const int seen_all = max(0, base + col0 / G), seen_any = max(0, base + (min(cols, col0 + 16 * CT) - 1) / G);
   const int tiles = (seen_any + 31) >> 5, per = (tiles + p.n_split - 1) / p.n_split, tile0 = sp * per, tile1 = min(tiles, tile0 + per);
 

@@ -708,7 +708,7 @@ int grove_kv4_read(const grove_kv4_read_params* p, void* stream);
 /* Causal attention of the new tokens of every request over its pages (its own rows appended before). q: bf16 [rows, heads, hd],
  * query head j reads key / value head j / (heads / kv); out: bf16 [rows, heads * hd].
  *   row r = cu_q[b] + i of request b with n = cu_q[b + 1] - cu_q[b] new tokens sees the keys t < kv_len[b] - n + i + 1:
- *   out[r] = softmax(alpha * q[r] . K[t]) V, fp32 throughout; 0 where it sees none.
+ *   out[r] = softmax(alpha * q[r] . K[t]) V, fp32 throughout; 0 where it sees none. Where cu_q passes `rows`, the rows that there are.
  * Keys whose table entry is outside [0, pages) are not seen. kv_len is cut to max_pages * page. Rows of no request are left as they
  * were; so are all with requests or max_q 0. n does not pass max_q (a request's rows past it become NaN), a row of the table not 2^30 tokens,
  * rows * heads not 2^30, nor 2^24 with more than 8 splits. q and its strides are aligned to 16 bytes, out and its row stride to 4. Rows of the

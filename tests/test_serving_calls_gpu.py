@@ -96,3 +96,17 @@ def test_attn_values_to_two_to_the_64(dev, H, kv, new, hd, max_len):
         o = ops.kv4_attn((q / ks).to(bf16).to(dev), c.cache, c.table, kv_len, cu, new, 1.0, max_len=max_len)
         res.append(o[:new].double() / vs)
     assert res[0].isfinite().all() and torch.equal(res[0], res[1]) and torch.equal(res[0], res[2])
+
+
+# ----------------------------------------------------------------------------- fewer rows than cu_q says
+@pytest.mark.parametrize("max_len", [1, 100000])
+@pytest.mark.parametrize("H,kv,new,hd", [s for s in SHAPES if s[2] > 1])
+def test_attn_rows_cut_short(dev, H, kv, new, hd, max_len):
+    """A step of fixed size that the last request's tokens pass (page_tables writes the rows that there are): those that are there keep their limits."""
+    from grove_amd import ops
+    lens = [20, 70, 9]
+    c, q, cu, kv_len, out = check_attn(dev, lens, [new, new, new], H, kv, hd, 16, seed=hd + 5, max_len=max_len)
+    qd = q.to(dev)
+    for rows in (2 * new, 2 * new - 1, new + 1, 1):
+        r = ops.kv4_attn(qd[:rows], c.cache, c.table, kv_len, cu, new, hd ** -0.5, max_len=max_len)
+        assert torch.equal(r, out[:rows]), rows
