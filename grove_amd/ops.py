@@ -1500,11 +1500,15 @@ def kv4_attn(q, cache, table, kv_len, cu_q, max_q, alpha, *, max_len=None, out=N
             _refuse(what, f"out must be bf16 [{rows}, {heads * hd}], its rows contiguous and apart")
         if not all(_apart(out, t) for t in (q, codes, scales, table, kv_len, cu_q)):
             _refuse(what, "out overlaps an input")
-        orow = out.stride(0)
+        orow = out.stride(0) if rows > 1 else heads * hd
         if orow % 2 or out.data_ptr() % 4:
             _refuse(what, "out must be aligned to 4 bytes, its row stride even")
-    if (qr % 8 and rows > 1) or qh % 8 or q.data_ptr() % 16:  # (an odd start or stride: its rows are laid out anew)
-        q = q.contiguous()
+    if rows == 1:  # (a stride that nothing is reached by)
+        qr = heads * hd
+    if heads == 1:
+        qh = hd
+    if qr % 8 or qh % 8 or q.data_ptr() % 16:  # (an odd start or stride: its rows are laid out anew, contiguous or not)
+        q = q.clone(memory_format=torch.contiguous_format)
         qr, qh = heads * hd, hd
     n_split = _kv4_split(B * kv, most * P if max_len is None else max_len, min(max_q, rows) * (heads // kv), hd)
     # the joined splits' workspace: from the allocator at every call, so that calls on other streams and captured graphs have their own

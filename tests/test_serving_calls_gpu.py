@@ -110,3 +110,24 @@ def test_attn_rows_cut_short(dev, H, kv, new, hd, max_len):
     for rows in (2 * new, 2 * new - 1, new + 1, 1):
         r = ops.kv4_attn(qd[:rows], c.cache, c.table, kv_len, cu, new, hd ** -0.5, max_len=max_len)
         assert torch.equal(r, out[:rows]), rows
+
+
+# ----------------------------------------------------------------------------- where q lies
+@pytest.mark.parametrize("rows", [1, 2, 5])
+@pytest.mark.parametrize("start", [0, 1, 4, 8])
+def test_attn_q_at_any_start(dev, rows, start):
+    """One row or several, contiguous or columns of a wider activation, at any start; and an output row with an odd stride."""
+    from grove_amd import ops
+    H, kv, hd = 4, 2, 64
+    c, q, cu, kv_len, ref = check_attn(dev, [70], [rows], H, kv, hd, 16, seed=rows)
+    flat = torch.full((start + rows * H * hd,), math.nan, dtype=bf16, device=dev)
+    flat[start:] = q.to(dev).flatten()
+    wide = torch.full((rows, H * hd + 3 + start), math.nan, dtype=bf16, device=dev)
+    wide[:, start:start + H * hd] = q.to(dev).flatten(1)
+    odd = wide[:, start:].as_strided((rows, H, hd), (wide.stride(0), hd, 1), start)
+    for x in (flat[start:].view(rows, H, hd), wide[:, start:start + H * hd].unflatten(1, (H, hd)), odd):
+        assert torch.equal(ops.kv4_attn(x, c.cache, c.table, kv_len, cu, rows, hd ** -0.5), ref)
+    if rows == 1:
+        out = torch.full((1, H * hd + 3), 5.0, dtype=bf16, device=dev)
+        ops.kv4_attn(q.to(dev), c.cache, c.table, kv_len, cu, 1, hd ** -0.5, out=out[:, :H * hd])
+        assert torch.equal(out[:, :H * hd], ref) and (out[:, H * hd:] == 5).all()

@@ -55,3 +55,46 @@ def test_attn_entry_takes_shared_table_rows():
     for ld, text in ((0, "null"), (1, "null"), (-4, "bad shape")):
         p = _lib.Kv4AttnParams(**fields, ld_table=ld)
         assert _lib.lib().grove_kv4_attn(ctypes.byref(p), None) == -1 and text in _lib.last_error(), ld
+
+
+# ----------------------------------------------------------------------------- q
+def packed(rows, width, start):
+    """[rows, 4, 64] as columns of a wider activation."""
+    return torch.randn(rows, width).to(bf16)[:, start:start + 256].unflatten(1, (4, 64))
+
+
+def flat(rows, start):
+    """A contiguous q that starts `start` elements behind an aligned address."""
+    return torch.randn(start + rows * 256).to(bf16)[start:].view(rows, 4, 64)
+
+
+@pytest.mark.parametrize("q,in_place", [
+    (flat(3, 0), True), (flat(3, 1), False), (flat(1, 3), False), (flat(3, 8), True), (packed(3, 512, 8), True), (packed(3, 259, 0), False), (packed(3, 512, 1), False),
+    (packed(1, 259, 0), True), (packed(1, 259, 3), False), (packed(1, 512, 8), True),
+    (torch.randn(3, 4, 67).to(bf16)[..., :64], False), (torch.randn(1, 1, 4, 67).to(bf16)[0, ..., :64], False),
+    (torch.randn(1, 256).to(bf16).as_strided((1, 4, 64), (3, 64, 1)), True), (torch.randn(1, 4, 64).to(bf16).expand(3, 4, 64), True)])
+def test_attn_q_reaches_the_entry_aligned(launched, q, in_place):
+    """Any start and any strides: read in place where the entry can, laid out anew elsewhere; what arrives are q's values."""
+    rows = q.shape[0]
+    attn(q, torch.zeros(3, 5, dtype=i32), rows_of=(1,) * rows + (0,) * (3 - rows))
+    (_, p, (got, *_)), = launched
+    assert p.q == got.data_ptr() and p.q % 16 == 0 and p.sq_row % 8 == 0 and p.sq_head % 8 == 0
+    assert (got.data_ptr() == q.data_ptr()) == in_place
+    assert torch.equal(got, q) and (rows == 1 or got.stride(0) == p.sq_row) and got.stride(1) == p.sq_head
+
+
+def test_attn_one_head_and_odd_head_stride(launched):
+    c = ops.kv4_cache(4, 16, 1, 64, "cpu")
+    q = torch.randn(2, 64).to(bf16).as_strided((2, 1, 64), (64, 3, 1))
+    ops.kv4_attn(q, c, torch.zeros(2, 5, dtype=i32), ints(3, 3), ints(0, 1, 2), 1, 1.0)
+    (_, p, (got, *_)), = launched
+    assert p.sq_head % 8 == 0 and torch.equal(got, q)
+
+
+def test_attn_out_of_one_row(launched):
+    """The stride of a single row is never used: any is taken."""
+    c = ops.kv4_cache(4, 16, 2, 64, "cpu")
+    out = torch.zeros(1, 259, dtype=bf16)[:, :256]
+    assert ops.kv4_attn(flat(1, 0), c, torch.zeros(1, 5, dtype=i32), ints(3), ints(0, 1), 1, 1.0, out=out) is out
+    (_, p, _), = launched
+    assert p.out == out.data_ptr() and p.so_row % 2 == 0
