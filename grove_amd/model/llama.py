@@ -258,7 +258,15 @@ class LlamaStack:
         """The pages of a 4-bit cache that requests of unlike lengths share, one ops.KV4Cache per layer: 3.8 times the tokens of new_kv_cache in
         the same memory at head_dim 128."""
         d = self.d
+        self._plain_plan()
         return [ops.kv4_cache(pages, page_size, d.n_heads, d.head_dim, self.dev) for _ in self.layers]
+
+    def _plain_plan(self):
+        """The model's own rotary plan, made with the first cache: its copy from the host must not fall into a captured step."""
+        plan = getattr(self, "_rotary_plan", None)
+        if plan is None:
+            plan = self._rotary_plan = ops.rotary_plan(self.d.head_dim, self.d.rope_theta, device=self.dev)
+        return plan
 
     def paged_step(self, x, step, table, cache, max_q, plan=None, max_len=None):
         """One serving step over the paged 4-bit cache: x bf16 [rows, H] = the embeddings of every request's new tokens, packed (a prompt or a piece
@@ -268,9 +276,7 @@ class LlamaStack:
         d = self.d
         nh, hd, I = d.n_heads, d.head_dim, d.mlp
         if plan is None:
-            plan = getattr(self, "_rotary_plan", None)
-            if plan is None:
-                plan = self._rotary_plan = ops.rotary_plan(hd, d.rope_theta, device=self.dev)
+            plan = self._plain_plan()
         T = x.shape[0]
         f32 = self.fp32_stream
         res = ops.to_f32(x) if f32 else None

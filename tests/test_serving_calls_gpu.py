@@ -131,3 +131,50 @@ def test_attn_q_at_any_start(dev, rows, start):
         out = torch.full((1, H * hd + 3), 5.0, dtype=bf16, device=dev)
         ops.kv4_attn(q.to(dev), c.cache, c.table, kv_len, cu, 1, hd ** -0.5, out=out[:, :H * hd])
         assert torch.equal(out[:, :H * hd], ref) and (out[:, H * hd:] == 5).all()
+
+
+# ----------------------------------------------------------------------------- the decoder stack, captured
+@pytest.mark.parametrize("stream", [f32, bf16])
+def test_paged_step_captured(dev, stream):
+    """Tables and the decoder stack in one captured step with rows of padding, the stack's own plan used there first: replayed over several steps,
+    with eager work between, against the eager step on a cache of its own."""
+    from grove_amd import ops
+    from grove_amd.model.llama import LlamaStack
+    from grove_amd.synthetic import TINY, synthetic_state_dict
+    d, P, T, B = TINY, 16, 9, 3
+    sd = {k: v.to(dev).to(bf16) for k, v in synthetic_state_dict(d).items() if k.startswith(("model.layers", "model.norm"))}
+    stack = LlamaStack(sd, d, dev, fp32_stream=stream == f32)
+    caches = [stack.new_kv4_cache(20, P) for _ in range(2)]
+    free = torch.randperm(20, generator=gen(1)).to(i32).to(dev)
+    state = [dict(table=torch.full((B, 5), -1, dtype=i32, device=dev), held=torch.zeros(B, dtype=i32, device=dev), free=free.clone()) for _ in range(2)]
+    x, ctx, new = torch.zeros(T, d.hidden, dtype=bf16, device=dev), torch.zeros(B, dtype=i32, device=dev), torch.zeros(B, dtype=i32, device=dev)
+
+    def body(i, plan=None):
+        s = state[i]
+        step = ops.page_tables(ctx, new, s["table"], s["held"], s["free"], P, T)
+        return step, stack.paged_step(x.clone(), step, s["table"], caches[i], 4, plan=plan)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):  # (nothing to be written: no request has a token; another plan, so that the stack's own is first used in the graph)
+        body(0, ops.rotary_plan(d.head_dim, device=dev))
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        res = body(0)
+    have = [0] * B
+    for i, n in enumerate([[4, 4, 1], [4, 0, 3], [1, 1, 1], [2, 3, 4], [1, 4, 4], [0, 1, 0]]):
+        x.copy_((torch.randn(T, d.hidden, generator=gen(30 + i)) * 0.5).to(bf16))
+        ctx.copy_(torch.tensor(have, dtype=i32))
+        new.copy_(torch.tensor(n, dtype=i32))
+        graph.replay()
+        got = [t.clone() for t in (*res[0], res[1])]
+        ref = body(1)
+        torch.cuda.synchronize()
+        for a, b in zip(got[:-1], ref[0]):
+            assert torch.equal(a, b), i
+        assert torch.equal(got[-1], ref[1]) and got[-1][:sum(n)].isfinite().all(), i
+        for s, step in zip(state, (res[0], ref[0])):
+            taken = int(step.taken)
+            s["free"].copy_(torch.roll(s["free"], -taken))
+            s["held"].copy_(step.held)
+        have = [a + b for a, b in zip(have, n)]

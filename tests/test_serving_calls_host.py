@@ -98,3 +98,17 @@ def test_attn_out_of_one_row(launched):
     assert ops.kv4_attn(flat(1, 0), c, torch.zeros(1, 5, dtype=i32), ints(3), ints(0, 1), 1, 1.0, out=out) is out
     (_, p, _), = launched
     assert p.out == out.data_ptr() and p.so_row % 2 == 0
+
+
+# ----------------------------------------------------------------------------- the decoder stack
+def test_stack_has_its_plan_before_the_first_step(monkeypatch):
+    """The plain plan is copied from the host; the first paged_step may be a captured one, in which such a copy is an error."""
+    from grove_amd.model.llama import LlamaStack
+    from grove_amd.synthetic import TINY
+    stack = LlamaStack.__new__(LlamaStack)
+    stack.d, stack.dev, stack.layers, stack.norm, stack.fp32_stream = TINY, "cpu", [], None, False
+    cache = stack.new_kv4_cache(2, 16)
+    monkeypatch.setattr(ops, "rotary_plan", lambda *a, **kw: pytest.fail("a plan is made within the step"))
+    monkeypatch.setattr(ops, "rmsnorm", lambda x, *a, **kw: x)
+    x = torch.zeros(1, TINY.hidden, dtype=bf16)
+    assert stack.paged_step(x, None, None, cache, 1) is x
