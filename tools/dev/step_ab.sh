@@ -4,9 +4,10 @@
 if [ "$1" = build ]; then
   set -e
   cd /root/repo/grove_amd/csrc
+  FLAGS=$(make -s flags)
   OBJS=$(ls build/*.o | grep -v "build/gemm.o\|build/gemm_tn.o\|_dbg\|_abl\|_drain\|_nd")
-  /opt/rocm/bin/hipcc -O3 -fPIC -std=c++17 --offload-arch=gfx950 -Wno-unused-value -Wno-unused-result -DPP_NO_EPI_DRAIN -c gemm.hip -o build/gemm_nd.o &
-  /opt/rocm/bin/hipcc -O3 -fPIC -std=c++17 --offload-arch=gfx950 -Wno-unused-value -Wno-unused-result -DTN_NO_EPI_DRAIN -c gemm_tn.hip -o build/gemm_tn_nd.o &
+  /opt/rocm/bin/hipcc $FLAGS -DPP_NO_EPI_DRAIN -c gemm.hip -o build/gemm_nd.o &
+  /opt/rocm/bin/hipcc $FLAGS -DTN_NO_EPI_DRAIN -c gemm_tn.hip -o build/gemm_tn_nd.o &
   wait
   /opt/rocm/bin/hipcc -shared -fPIC --offload-arch=gfx950 -o libgrove_hip_nodrain.so $OBJS build/gemm_nd.o build/gemm_tn_nd.o
   ls -la libgrove_hip_nodrain.so

@@ -1,6 +1,6 @@
 """Checks the compiled gemm_nt_w4_kernel instances: outside the hand-written asm statements the compiler must not touch the
 accumulator AGPRs at all, and must not touch the fragment VGPRs v128..v255 in any block of the K loop (between two bodies).
-Usage: python tools/gen/check_w4_isa.py gemm.s   (gemm.s = hipcc -S --cuda-device-only of grove_amd/csrc/gemm.hip)"""
+Usage: python tools/gen/check_w4_isa.py gemm.s   (gemm.s = hipcc $(make -s -C grove_amd/csrc flags) -S --cuda-device-only of grove_amd/csrc/gemm.hip)"""
 import re
 import sys
 

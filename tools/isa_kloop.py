@@ -1,7 +1,7 @@
 """Offline ISA check of the persistent GEMM instances (no GPU needed): per gemm_nt_pp_kernel instance, total s_waitcnt vmcnt(0), scratch
 ops, 128-bit LDS ops and — per K-loop body (runs of MFMAs) — the vmcnt(0) waits INSIDE it (the baseline has the four explicit tail waits;
 anything more is hipcc guarding LDS reads / reloading spilled staging pointers, i.e. the staging queue drained once per tile).
-    hipcc -O3 -std=c++17 --offload-arch=gfx950 -S --cuda-device-only -Iinclude grove_amd/csrc/gemm.hip -o /tmp/gemm.s && python tools/isa_kloop.py /tmp/gemm.s"""
+    hipcc $(make -s -C grove_amd/csrc flags) -S --cuda-device-only grove_amd/csrc/gemm.hip -o /tmp/gemm.s && python tools/isa_kloop.py /tmp/gemm.s"""
 import re,sys
 lines=open(sys.argv[1]).read().split('\n')
 starts=[(i,l.split(':')[0]) for i,l in enumerate(lines) if re.match(r'^_Z.*gemm_nt_pp_kernel.*:\s*;',l)]

@@ -4,7 +4,7 @@ edge into the K loop — runs in EVERY iteration, and with LDS-DMA pieces in the
 drained once per K tile. Round 5 found one in gemm_tn_pp_kernel (3 % of the kernel) and one in the 256-row GELU instance of
 gemm_nt_pp_kernel (7 %). Waits written by the source (inside ;;#ASMSTART ... ;;#ASMEND) are not reported; by default only loops that
 issue LDS-DMA are (register-staged kernels need their waits; --all lists those too).
-    hipcc -O3 -std=c++17 --offload-arch=gfx950 -S --cuda-device-only grove_amd/csrc/X.hip -o /tmp/X.s && python tools/isa_loop_waits.py /tmp/X.s"""
+    hipcc $(make -s -C grove_amd/csrc flags) -S --cuda-device-only grove_amd/csrc/X.hip -o /tmp/X.s && python tools/isa_loop_waits.py /tmp/X.s"""
 import re
 import sys
 

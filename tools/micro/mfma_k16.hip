@@ -5,7 +5,7 @@
 // Register-only loops, one block of 512 threads per CU (2 waves per SIMD), 8 independent accumulators per wave:
 //   a: 16x16x32                       b: 2 x 16x16x16 per 32-deep step (same FLOPs)
 //   c: 16x16x32 + 4 v_mov per MFMA    d: 2 x 16x16x16 (+ 0 v_mov)      e: 16x16x32 + 2 v_mov per MFMA
-// prints us per launch and TFLOP/s.   hipcc --offload-arch=gfx950 -O3 mfma_k16.hip -o mfma_k16
+// prints us per launch and TFLOP/s.   hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops mfma_k16.hip -o mfma_k16
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #include <cstdlib>

@@ -1,7 +1,7 @@
 // What does the matrix pipe sustain under the board's power limit, and does the MFMA block shape matter? Register-only loops (no LDS, no
 // memory): 8 waves per CU on every CU, operands = normally distributed bf16 values loaded once, 8 (16x16x32) or 4 (32x32x16) independent
 // accumulators per wave so that the pipe never waits on a dependency. Each variant runs for ~3 s; prints TFLOP/s and the implied clock
-// (TFLOP/s / (256 CUs * 4 SIMDs * 1024 FLOP per clock)).   hipcc --offload-arch=gfx950 -O3 mfma_power.hip -o mfma_power
+// (TFLOP/s / (256 CUs * 4 SIMDs * 1024 FLOP per clock)).   hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops mfma_power.hip -o mfma_power
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #include <cstdlib>

@@ -4,7 +4,7 @@
 //   B  lane -> (row lane >> 3 [+ 8], 16 bytes at 128 u + 16 (lane & 7)): 128 contiguous bytes per row per instruction, two instructions per 16 rows
 //   C  the same bytes per instruction as B with the lanes of a row STRIDED: lane -> (row lane & 7 [+ 8], chunk 4 ((lane >> 3) & 1) + (lane >> 4)) —
 //      one lane-pair exchange away from the MFMA operand layout
-// hipcc --offload-arch=gfx950 -O3 tools/micro/row_request_shape.hip -o tools/micro/row_request_shape && tools/micro/row_request_shape
+// hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops tools/micro/row_request_shape.hip -o tools/micro/row_request_shape && tools/micro/row_request_shape
 #include <hip/hip_runtime.h>
 #include <stdio.h>
 #include <vector>

@@ -1,6 +1,6 @@
 // Per-CU store-path microbenchmark: one 512-thread block per CU writes 256 x 256 bf16 tiles (128 KB) of a row-major matrix
 // with different lane -> address patterns. Answers: is the GEMM epilogue bound by bytes or by the number of write requests?
-//   hipcc --offload-arch=gfx950 -O3 -o /tmp/store_bw tools/micro/store_bw.hip && /tmp/store_bw
+//   hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops -o /tmp/store_bw tools/micro/store_bw.hip && /tmp/store_bw
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #include <cstdint>
