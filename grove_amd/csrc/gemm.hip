@@ -421,11 +421,14 @@ constexpr int P_STAGE = 4 * P_HALF;              // A_lo | B_lo | B_hi | A_hi (s
 // the 16 stores take under 2000 — so: one 64-bit row pointer per A half, uniform (scalar) row steps, and every residual
 // load issued before a store it would otherwise queue behind (vmcnt retires in order):
 //   loads(h0) compute(h0) loads(h1) stores(h0) compute(h1) stores(h1)
-template <int MIH, int BMH, int ACT>
+// RES: 1 / 0 = a residual is there / is not, known at compile time (-1: tested here). Where the loads of the residual and their use hang on
+// two tests of p.residual, hipcc sees a path on which the loads stay pending, and waits for them wherever the registers are used next.
+template <int MIH, int BMH, int ACT, int RES = -1>
 __device__ __forceinline__ void gemm_epilogue_fast(const grove_gemm_params& p, f32x4_t (&acc)[2 * MIH][4], const int mw0, const int nw0,
                                                    const int fr, const int fq, const float scale) {
   constexpr bool PLAIN = ACT < 0;
   constexpr bool PAIR = ACT == GROVE_ACT_SWIGLU_PAIR;
+  const bool has_res = RES < 0 ? p.residual != nullptr : RES != 0;
   const int n0 = nw0 + fq * 8;  // column group 0; group 1 is 128 columns on
   const int64_t row0 = mw0 + fr;
   float bv[2][8];
@@ -485,14 +488,23 @@ __device__ __forceinline__ void gemm_epilogue_fast(const grove_gemm_params& p, f
           for (int e = 0; e < 4; ++e) o[e] = gg[e] * fast_sigmoid(gg[e]) * uu[e];
           outp[i][g] = u32x4_t{pack2bf(o[0], o[1]), pack2bf(o[2], o[3]), 0u, 0u};
         } else {
-          if (ap && p.aux_grad) {  // aux = act'(v): computed together with act(v)
+          if constexpr (ACT == GROVE_ACT_RELU) {  // (shares nothing with its derivative: aux first, so that v and relu(v) are not both held: 48 spilled registers less)
+            if (ap) {
+              float av[8];
+#pragma unroll
+              for (int e = 0; e < 8; ++e) av[e] = p.aux_grad ? act_grad(ACT, v[e]) : v[e];
+              *(u32x4_t*)(ap + (int64_t)(i * 16) * ld_aux + g * 128) =
+                  u32x4_t{pack2bf(av[0], av[1]), pack2bf(av[2], av[3]), pack2bf(av[4], av[5]), pack2bf(av[6], av[7])};
+            }
+          }
+          if (ACT != GROVE_ACT_RELU && ap && p.aux_grad) {  // aux = act'(v): computed together with act(v)
             float av[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) act_apply_grad(ACT < 0 ? GROVE_ACT_NONE : ACT, v[e], v[e], av[e]);
             *(u32x4_t*)(ap + (int64_t)(i * 16) * ld_aux + g * 128) =
                 u32x4_t{pack2bf(av[0], av[1]), pack2bf(av[2], av[3]), pack2bf(av[4], av[5]), pack2bf(av[6], av[7])};
           } else {
-            if (ap)
+            if (ACT != GROVE_ACT_RELU && ap)
               *(u32x4_t*)(ap + (int64_t)(i * 16) * ld_aux + g * 128) =
                   u32x4_t{pack2bf(v[0], v[1]), pack2bf(v[2], v[3]), pack2bf(v[4], v[5]), pack2bf(v[6], v[7])};
             if (!PLAIN && ACT != GROVE_ACT_NONE) {
@@ -504,11 +516,14 @@ __device__ __forceinline__ void gemm_epilogue_fast(const grove_gemm_params& p, f
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[e] *= scale;
           }
-          if (p.residual) {
+          if (has_res) {
             const u32x4_t q = rr[i][g];
             const float rv[8] = {bf_lo(q.x), bf_hi(q.x), bf_lo(q.y), bf_hi(q.y), bf_lo(q.z), bf_hi(q.z), bf_lo(q.w), bf_hi(q.w)};
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = p.residual_mul ? v[e] * rv[e] : v[e] + rv[e];
+            for (int e = 0; e < 8; ++e) {
+#pragma clang fp contract(off)  // (the scaled value is rounded before the sum, as in the other instances and at a tile on the edge)
+              v[e] = p.residual_mul ? v[e] * rv[e] : v[e] + rv[e];
+            }
           }
           outp[i][g] = u32x4_t{pack2bf(v[0], v[1]), pack2bf(v[2], v[3]), pack2bf(v[4], v[5]), pack2bf(v[6], v[7])};
         }
@@ -524,9 +539,9 @@ __device__ __forceinline__ void gemm_epilogue_fast(const grove_gemm_params& p, f
         else *(u32x4_t*)(cp + (int64_t)(i * 16) * p.ldc + g * 128) = outp[i][g];
       }
   };
-  if (p.residual) load_res(0);
+  if (has_res) load_res(0);
   compute(0);
-  if (p.residual) load_res(1);
+  if (has_res) load_res(1);
   store(0);
   compute(1);
   store(1);
@@ -621,7 +636,17 @@ __device__ __forceinline__ void gemm_epilogue_wide(const grove_gemm_params& p, f
           outp[i][g] = u32x4_t{pack2bf(o[0], o[1]), pack2bf(o[2], o[3]), 0u, 0u};
           continue;
         }
-        if (p.aux && p.aux_grad) {  // aux = act'(v): computed together with act(v)
+        if constexpr (ACT == GROVE_ACT_RELU) {  // see gemm_epilogue_fast
+          if (p.aux) {
+            float av[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) av[e] = p.aux_grad ? act_grad(ACT, v[e]) : v[e];
+            if (ok)
+              *(u32x4_t*)((bf16_raw*)p.aux + (int64_t)crow[i] * (p.ld_aux ? p.ld_aux : p.ldc) + n) =
+                  u32x4_t{pack2bf(av[0], av[1]), pack2bf(av[2], av[3]), pack2bf(av[4], av[5]), pack2bf(av[6], av[7])};
+          }
+        }
+        if (ACT != GROVE_ACT_RELU && p.aux && p.aux_grad) {  // aux = act'(v): computed together with act(v)
           float av[8];
 #pragma unroll
           for (int e = 0; e < 8; ++e) act_apply_grad(ACT < 0 ? GROVE_ACT_NONE : ACT, v[e], v[e], av[e]);
@@ -629,7 +654,7 @@ __device__ __forceinline__ void gemm_epilogue_wide(const grove_gemm_params& p, f
             *(u32x4_t*)((bf16_raw*)p.aux + (int64_t)crow[i] * (p.ld_aux ? p.ld_aux : p.ldc) + n) =
                 u32x4_t{pack2bf(av[0], av[1]), pack2bf(av[2], av[3]), pack2bf(av[4], av[5]), pack2bf(av[6], av[7])};
         } else {
-          if (p.aux && ok)
+          if (ACT != GROVE_ACT_RELU && p.aux && ok)
             *(u32x4_t*)((bf16_raw*)p.aux + (int64_t)crow[i] * (p.ld_aux ? p.ld_aux : p.ldc) + n) =
                 u32x4_t{pack2bf(v[0], v[1]), pack2bf(v[2], v[3]), pack2bf(v[4], v[5]), pack2bf(v[6], v[7])};
           if (!PLAIN && ACT != GROVE_ACT_NONE && !PAIR) {
@@ -685,7 +710,9 @@ __device__ __forceinline__ void gemm_epilogue_wide(const grove_gemm_params& p, f
         for (int i = 0; i < MIH; ++i) {
           if (crow[i] < 0) continue;
           bf16_raw* c = (bf16_raw*)p.C + (int64_t)crow[i] * p.ldc + n + ngrp * p.n_pad + 8;
-          for (int z = 0; z < p.n_pad; z += 8) *(u32x4_t*)(c + z) = u32x4_t{0u, 0u, 0u, 0u};
+          unsigned zero;  // (made here: as a constant hipcc keeps four registers of it through the K loops)
+          asm volatile("v_mov_b32 %0, 0" : "=v"(zero));
+          for (int z = 0; z < p.n_pad; z += 8) *(u32x4_t*)(c + z) = u32x4_t{zero, zero, zero, zero};
         }
       }
     }
@@ -1141,6 +1168,9 @@ __global__ __launch_bounds__(P_NT) void gemm_nt_pp_kernel(const grove_gemm_param
     }
   };
   const bool fast_addr = p.c_dtype == GROVE_BF16 && !p.c_idx && !p.r_idx && !p.n_group;  // gemm_epilogue_fast's case
+  // the instances whose K loops got a wait otherwise: scaled, (32768, 5120, 1280) 399 -> 374 us; gathered and scaled, K = 34560, 2045 -> 1915 (the
+  // gathered ReLU one had them where a tap ends, and takes the same time)
+  constexpr bool SPLIT_RES = !FP8 && BM == 256 && (ACT == GROVE_ACT_NONE || (GATHER && ACT == GROVE_ACT_RELU));
   // my output tiles in turn: their K tiles (STEADY while the stream still has a half-tile to issue six phases ahead, i.e. all
   // but the stream's last two), then the epilogue (no barriers inside) — the next tile's operands are already landing
   int T = 0;
@@ -1184,7 +1214,8 @@ __global__ __launch_bounds__(P_NT) void gemm_nt_pp_kernel(const grove_gemm_param
       const bool interior = fast_addr && m0 + BM <= p.M && n0 + P_BN <= p.N;
       if constexpr (FP8) fp8_scale_acc<MIH, BMH>(p, work, acc, mw0, nw0, fr, fq);
       if constexpr (ACT == GROVE_ACT_SWIGLU_BWD) gemm_epilogue_swiglu_bwd<MIH, BMH>(p, acc, mw0, nw0, fr, fq);
-      else if (interior) gemm_epilogue_fast<MIH, BMH, ACT>(p, acc, mw0, nw0, fr, fq, ACT < 0 ? 1.f : scale);
+      else if (interior && SPLIT_RES && p.residual) gemm_epilogue_fast<MIH, BMH, ACT, 1>(p, acc, mw0, nw0, fr, fq, ACT < 0 ? 1.f : scale);
+      else if (interior) gemm_epilogue_fast<MIH, BMH, ACT, SPLIT_RES ? 0 : -1>(p, acc, mw0, nw0, fr, fq, ACT < 0 ? 1.f : scale);
       else gemm_epilogue_wide<MIH, BMH, ACT>(p, acc, mw0, nw0, fr, fq, ACT < 0 ? 1.f : scale);
       relax = interior && !p.aux && !FP8 && ACT != GROVE_ACT_SWIGLU_BWD;  // exactly 4 * MIH stores per wave were issued (FP8: the scale loads sit in the queue too)
       // Round 5: in the 256-row GELU instance (SAM's fc1: 32 launches, 15 ms per step) hipcc's register allocation leaves epilogue
