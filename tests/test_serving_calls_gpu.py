@@ -178,3 +178,31 @@ def test_paged_step_captured(dev, stream):
             s["free"].copy_(torch.roll(s["free"], -taken))
             s["held"].copy_(step.held)
         have = [a + b for a, b in zip(have, n)]
+
+
+# ----------------------------------------------------------------------------- verification, one launch and two
+@pytest.mark.parametrize("dtype", [f32, bf16])
+@pytest.mark.parametrize("V", [50, 9001, 32008, 1100003])  # one block, several per request, chunks of more than 1024
+def test_verify_edges_at_every_vocabulary(dev, dtype, V):
+    B, K = 5, 3
+    d, q, p, u, pick = drafts(B, K, V, V, dtype)
+    bad = d.clone()
+    bad[0, 0], bad[1, 1], bad[2, 2], bad[4, 0] = -1, V, 2 ** 31 - 1, V + 7       # tokens that do not exist: refused
+    same = p[:, :K].clone()
+    t = check_verify(dev, bad, same, p, u, pick)                                # ... where p - q leaves nothing: drawn from p itself
+    assert (t[:3] >= -1).all() and (t[[0, 4], 0] >= 0).all() and (t[1, 1] >= 0) and (t[2, 2] >= 0)
+    less = same.clone()
+    less[4, 0, V // 3] = 0                                                      # ... and where it leaves one token
+    assert check_verify(dev, bad, less, p, u, pick)[4, 0] == V // 3
+    check_verify(dev, bad, q, p, u, pick)
+    check_verify(dev, bad, None, p, u, pick)
+    for a in (0.0, 1 - 2.0 ** -24):
+        for b in (0.0, 1 - 2.0 ** -24):
+            check_verify(dev, bad, q, p, torch.full_like(u, a), torch.full_like(pick, b))
+    zero = p.clone()
+    zero[1], zero[2, 1:] = 0, 0
+    t = check_verify(dev, bad, q, zero, u, pick)                                # no mass at all: no token
+    assert t[1, 0] == -1
+    one = torch.zeros_like(p)
+    one[..., V - 1] = 1
+    assert (check_verify(dev, bad, None, one, u, pick)[:, 0] == V - 1).all()     # certain of the last token
