@@ -206,3 +206,75 @@ def test_verify_edges_at_every_vocabulary(dev, dtype, V):
     one = torch.zeros_like(p)
     one[..., V - 1] = 1
     assert (check_verify(dev, bad, None, one, u, pick)[:, 0] == V - 1).all()     # certain of the last token
+
+
+# ----------------------------------------------------------------------------- the loop around a step
+def test_serving_loop_keeps_every_context(dev):
+    """Prompts in pieces, next tokens and drafts in the same steps, lengths carried on as ctx = kv_len - (count - accepted): after every step the
+    cache holds exactly the rows of each request's accepted tokens, at their positions, and the step's attention saw them."""
+    from grove_amd import ops
+    B, H, kv, hd, P, K, V = 4, 4, 2, 64, 16, 3, 40
+    g = gen(91)
+    emb = torch.randn(V, H + 2 * kv, hd, generator=g).to(bf16).to(dev)
+    plan = ops.rotary_plan(hd, device=dev)
+    cache = ops.kv4_cache(60, P, kv, hd, dev)
+    free, table = torch.randperm(60, generator=g).to(i32).to(dev), torch.full((B, 14), -1, dtype=i32, device=dev)
+    ctx, held = torch.zeros(B, dtype=i32, device=dev), torch.zeros(B, dtype=i32, device=dev)
+    prompts = [torch.randint(0, V, (n,), generator=g).tolist() for n in (37, 1, 50, 5)]
+    seqs, todo = [[] for _ in range(B)], [[p[:20], p[20:]] if len(p) > 20 else [p] for p in prompts]
+    nxt = [None] * B
+    for it in range(9):
+        new, count, draft = [], [], torch.zeros(B, K, dtype=i32)
+        for b in range(B):
+            if todo[b] and it >= b:  # (the requests come one after the other)
+                new.append(todo[b].pop(0))
+                count.append(0)
+            elif nxt[b] is None:
+                new.append([])
+                count.append(0)
+            else:
+                n = (it + b) % (K + 1)
+                draft[b, :n] = torch.randint(0, V, (n,), generator=g).to(i32)
+                new.append([nxt[b]] + draft[b, :n].tolist())
+                count.append(n)
+        T = sum(len(t) for t in new)
+        ids = torch.tensor(sum(new, []), device=dev)
+        cnt = torch.tensor(count, dtype=i32, device=dev)
+        step = ops.page_tables(ctx, torch.tensor([len(t) for t in new], dtype=i32, device=dev), table, held, free, P, T)
+        free, held = free[int(step.taken):], step.held
+        x = emb[ids]
+        ops.rotary(x[:, :H + kv], step.pos, plan, out=x[:, :H + kv])
+        ops.kv4_append(x[:, H:H + kv], x[:, H + kv:], cache, step.slots)
+        out = ops.kv4_attn(x[:, :H], cache, table, step.kv_len, step.cu_q, max(len(t) for t in new), hd ** -0.5)
+        rows = (step.cu_q[1:] - 1 - cnt)[:, None] + torch.arange(K + 1, device=dev)
+        z = torch.randn(T, V, generator=g).to(dev)
+        z[:, :12] += 2
+        p = torch.softmax(z, -1)[rows.clamp(0, T - 1)]
+        u, pick = torch.rand(B, K, generator=g).to(dev) * 0.05, torch.rand(B, generator=g).to(dev)
+        tokens, accepted = ops.verify_drafts(draft.to(dev), None, p, u, pick, cnt)
+        ctx = step.kv_len - (cnt - accepted)
+        ref = verify_ref(draft, None, p.cpu(), u.cpu(), pick.cpu(), cnt.cpu())
+        assert torch.equal(tokens.cpu(), ref[0]) and torch.equal(accepted.cpu(), ref[1])
+        want, whole = [], ops.kv4_cache(B * 14, P, kv, hd, dev)
+        for b in range(B):
+            full = seqs[b] + new[b]
+            a = int(accepted[b])
+            if new[b]:
+                seqs[b] = seqs[b] + new[b][:len(new[b]) - count[b] + a]
+                nxt[b] = int(tokens[b, a]) if not todo[b] else None
+            assert int(ctx[b]) == len(seqs[b]), (it, b)
+            want.append(full)
+        # the same contexts written at once into a cache of their own, pages in order
+        own = torch.arange(B * 14, dtype=i32, device=dev).view(B, 14)
+        for b, full in enumerate(want):
+            if full:
+                y, pos = emb[torch.tensor(full, device=dev)], torch.arange(len(full), dtype=i32, device=dev)
+                ops.rotary(y[:, :H + kv], pos, plan, out=y[:, :H + kv])
+                ops.kv4_append(y[:, H:H + kv], y[:, H + kv:], whole, b * 14 * P + pos)
+        assert torch.equal(out, ops.kv4_attn(x[:, :H], whole, own, step.kv_len, step.cu_q, max(len(t) for t in new), hd ** -0.5)), it
+        for b in range(B):
+            t = torch.arange(len(seqs[b]), device=dev)
+            at = (table[b, t // P] * P + t % P).to(i32)
+            for s, w in zip(ops.kv4_read(cache, at, f32), ops.kv4_read(whole, (b * 14 * P + t).to(i32), f32)):
+                assert torch.equal(s, w), (it, b)
+    assert sum(len(s) for s in seqs) > 100 and any(len(s) > len(p) + 4 for s, p in zip(seqs, prompts))
