@@ -1269,9 +1269,10 @@ class RotaryPlan(NamedTuple):
 
 def rotary_plan(rot, theta=10000.0, *, interleaved=False, scaling="none", factor=1.0, trained_len=4096, fast=32.0, slow=1.0, device="cuda"):
     """The frequencies theta^(-2 i / rot) of `rot` rotated channels, stretched by `factor` for contexts longer than `trained_len`:
-    "linear" divides every frequency; "ntk" raises theta to theta * factor^(rot / (rot - 2)), which divides the lowest frequency only; "yarn"
-    divides the pairs that turn less than `slow` times in trained_len, leaves those that turn more than `fast` times, blends linearly over
-    the pair number between, and scales the rotated channels by 0.1 ln(factor) + 1 (Peng et al. 2023)."""
+    "linear" divides every frequency; "ntk" raises theta to theta * factor^(rot / (rot - 2)), which divides frequency i by
+    factor^(2 i / (rot - 2)): the highest by 1, the lowest by factor; "yarn" (Peng et al. 2023) divides the pairs that turn less than `slow` times in
+    trained_len, leaves those that turn more than `fast` times, blends between, and scales the rotated channels by 0.1 ln(factor) + 1. The blend is linear in
+    the pair number, between whole ones, as checkpoints were trained with: from floor(p(fast)) to ceil(p(slow)), p(t) = the pair that turns t times."""
     what = "rotary_plan"
     if rot < 2 or rot % 2:
         _refuse(what, f"rot = {rot} must be even and positive")

@@ -1,5 +1,6 @@
 """What the serving operators hand to their C entries, with the launch replaced: no GPU needed."""
 import ctypes
+import math
 
 import pytest
 import torch
@@ -112,3 +113,27 @@ def test_stack_has_its_plan_before_the_first_step(monkeypatch):
     monkeypatch.setattr(ops, "rmsnorm", lambda x, *a, **kw: x)
     x = torch.zeros(1, TINY.hidden, dtype=bf16)
     assert stack.paged_step(x, None, None, cache, 1) is x
+
+
+# ----------------------------------------------------------------------------- stretched frequencies
+@pytest.mark.parametrize("rot,theta,factor,trained", [(64, 10000.0, 4.0, 4096), (128, 10000.0, 8.0, 2048), (128, 500000.0, 16.0, 8192), (32, 10000.0, 2.0, 512)])
+def test_plan_between_the_ends(rot, theta, factor, trained):
+    """Every frequency of the three scalings, pair by pair; yarn's blend between its ends too."""
+    base = [theta ** (-2 * i / rot) for i in range(rot // 2)]
+
+    def plan(kind):
+        return ops.rotary_plan(rot, theta, scaling=kind, factor=factor, trained_len=trained, device="cpu").freq.tolist()
+    for got, w in zip(plan("linear"), base):
+        assert math.isclose(got, w / factor, rel_tol=1e-12)
+    for i, (got, w) in enumerate(zip(plan("ntk"), base)):
+        assert math.isclose(got, w / factor ** (2 * i / (rot - 2)), rel_tol=1e-12)
+    # pair p turns trained * theta^(-2 p / rot) / (2 pi) times: the real p at which that is 32, and 1
+    fast, slow = (rot / 2 * math.log(trained / (2 * math.pi * t), theta) for t in (32.0, 1.0))
+    low, high = max(math.floor(fast), 0), math.ceil(slow)
+    assert 0 < high < rot - 1 and low < high
+    inside = 0
+    for i, (got, w) in enumerate(zip(plan("yarn"), base)):
+        part = min(max((i - low) / (high - low), 0.0), 1.0)
+        inside += 0 < part < 1
+        assert math.isclose(got, w * (1 - part) + w / factor * part, rel_tol=1e-12), i
+    assert inside >= 3
