@@ -1428,11 +1428,13 @@ def kv4_append(k, v, cache, slots):
     codes, scales = cache
     kp, vp, sp, c0, s0 = k.data_ptr(), v.data_ptr(), slots.data_ptr(), codes.data_ptr(), scales.data_ptr()
     c1, s1 = c0 + codes.numel(), s0 + 2 * scales.numel()
-    for a in (kp, vp, sp):
-        if c0 <= a < c1 or s0 <= a < s1:
-            _refuse(what, "an input lies in the cache")
     kr, kh, _ = k.stride()
     vr, vh, _ = v.stride()
+    if rows:
+        n, m = rows - 1, kv - 1
+        for a, e in ((kp, kp + 2 * (n * kr + m * kh + hd)), (vp, vp + 2 * (n * vr + m * vh + hd)), (sp, sp + 4 * rows)):
+            if (a < c1 and e > c0) or (a < s1 and e > s0):
+                _refuse(what, "an input lies in the cache")
     _launch(what, _pack_kv4append(kp, vp, c0, s0, sp, kr, kh, vr, vh, rows, kv, hd, P, pages), k, v, codes, scales, slots)
 
 

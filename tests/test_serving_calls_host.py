@@ -137,3 +137,22 @@ def test_plan_between_the_ends(rot, theta, factor, trained):
         inside += 0 < part < 1
         assert math.isclose(got, w * (1 - part) + w / factor * part, rel_tol=1e-12), i
     assert inside >= 3
+
+
+# ----------------------------------------------------------------------------- inputs that reach into the cache
+def test_append_input_that_ends_in_the_cache():
+    """A cache in one buffer with the rows before it: rows that run on into the codes are refused, rows that end where they begin are not."""
+    pages, kv, P, hd = 2, 1, 16, 32
+    codes, scales = pages * 2 * kv * P * hd // 2, pages * 2 * kv * P * 2
+    buf = torch.zeros(256 + codes + 2 * scales, dtype=torch.uint8)
+    c = ops.KV4Cache(buf[256:256 + codes].view(pages, 2, kv, P * hd // 2), buf[256 + codes:].view(bf16).view(pages, 2, kv, P, 2))
+    rows, slots = buf.view(bf16)[:128].view(4, 1, 32), torch.arange(4, dtype=i32)
+    over = buf.view(bf16)[32:160].view(4, 1, 32)
+    other = torch.zeros(4, 1, 32, dtype=bf16)
+    with pytest.raises(RuntimeError, match="need device tensors"):
+        ops.kv4_append(rows, other, c, slots)
+    for k, v in ((over, other), (other, over)):
+        with pytest.raises(RuntimeError, match="lies in the cache"):
+            ops.kv4_append(k, v, c, slots)
+    with pytest.raises(RuntimeError, match="lies in the cache"):
+        ops.kv4_append(other, other, c, buf[250:].view(torch.uint8)[2:18].view(i32))
