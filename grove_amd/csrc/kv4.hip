@@ -200,8 +200,9 @@ __global__ __launch_bounds__(256) void kv4_read_kernel(const grove_kv4_read_para
 //     4 h + i of either part in lane (col, h), and the values' four-token order gives the A operand the same keys. P s goes in as two bf16 parts
 //     (hi + lo, 2^-17), the minimum's share sum P (m - 16 s) is one number per column.
 // Bound, at hd 128: 32 contexts of up to 32768 keys under 4 heads a group, one token each (607 MB): 123 us and 4 for the join, 4.8 TB/s, what a large
-// copy reaches. 32 columns and more: by the vector instructions of the softmax (some 14 a score, four of them the exponential; 64 requests x 8 tokens x 4
-// heads over up to 4096 keys: 70 us for 156 MB). hd 64: by the same, at half the bytes a key (54 us for 161 MB). Few short contexts: by the chain
+// copy reaches. 32 columns and more: by ragged lengths and by the chain product, softmax, product of a tile with a wave or two on a SIMD (64 requests x 8
+// tokens x 4 heads over up to 4096 keys: 71 us for 167 MB, of which a wave lives half; vector units 37 % busy, matrix units 15; even lengths: 46 us).
+// hd 64 and 32: by the work per tile, at half and a quarter of the bytes (53 us for 168 MB, 45 for 93; vector units 57 %). Few short contexts: by the chain
 // lengths -> page -> tile -> output, 5 us, 7 with two column tiles, and 3 for the join (one context of 703 keys, 32 heads: 7.7 us in 8 blocks a head).
 // The tiles travel global -> LDS (LDS-DMA) into a ring of kv4_slots slots per wave: several tiles per wave are in flight without a register held
 // for them. At hd 128 and 256 every lane takes back the bytes that it asked for, side by side in lane order: no bank conflicts. No barriers: a wave

@@ -271,8 +271,9 @@ class LlamaStack:
     def paged_step(self, x, step, table, cache, max_q, plan=None, max_len=None):
         """One serving step over the paged 4-bit cache: x bf16 [rows, H] = the embeddings of every request's new tokens, packed (a prompt or a piece
         of it, the next token, or that and drafted ones: ops.verify_drafts takes the logits' probabilities); step: the ops.PageStep that
-        ops.page_tables made for these rows with `table`; cache: new_kv4_cache; max_q: the most new tokens of a request; plan: ops.rotary_plan for
-        contexts longer than trained (default: the plain one); max_len: ops.kv4_attn's. Returns the final-norm hidden rows [rows, H] (bf16)."""
+        ops.page_tables made for these rows with `table`; cache: new_kv4_cache; max_q: the most new tokens of a request, for which the
+        attention of every request is launched (a long prompt is best given a step of its own); plan: ops.rotary_plan for contexts longer than trained
+        (default: the plain one); max_len: ops.kv4_attn's. Returns the final-norm hidden rows [rows, H] (bf16)."""
         d = self.d
         nh, hd, I = d.n_heads, d.head_dim, d.mlp
         if plan is None:
