@@ -712,8 +712,9 @@ int grove_kv4_read(const grove_kv4_read_params* p, void* stream);
  * Keys whose table entry is outside [0, pages) are not seen. kv_len is cut to max_pages * page. Rows of no request are left as they
  * were; so are all with requests or max_q 0. n does not pass max_q (a request's rows past it become NaN), a row of the table not 2^30 tokens,
  * rows * heads not 2^30, nor 2^24 with more than 8 splits. q and its strides are aligned to 16 bytes, out and its row stride to 4. Rows of the
- * cache that no query sees may hold anything. Those that are seen: values up to 2^64 in size, and keys whose |alpha| sum|q| (31 s + |m|) stays below
- * 2^126 (s, m: the row's scale and minimum); beyond that a result may be infinite or NaN where the formula's is not, for the queries that see the row.
+ * cache that no query sees may hold anything. Of those that are seen, for finite results wherever the formula's are: values up to 2^64 in size, and per
+ * query sum|q| below 2^120 and |alpha| sum|q| (31 s + |m|) below 2^126 (s, m: a key row's scale and minimum). Beyond that the queries that see the row
+ * may get infinities or NaN.
  * n_split > 1 (at most 64): a request's keys are dealt to n_split blocks, whose partial results lie in `partial`, f32 [rows * heads * n_split *
  * (hd + 2)], and are joined by a second launch. Otherwise `partial` may be NULL. */
 typedef struct grove_kv4_attn_params {
