@@ -278,3 +278,22 @@ def test_serving_loop_keeps_every_context(dev):
             for s, w in zip(ops.kv4_read(cache, at, f32), ops.kv4_read(whole, (b * 14 * P + t).to(i32), f32)):
                 assert torch.equal(s, w), (it, b)
     assert sum(len(s) for s in seqs) > 100 and any(len(s) > len(p) + 4 for s, p in zip(seqs, prompts))
+
+
+# ----------------------------------------------------------------------------- queries that are no numbers
+@pytest.mark.parametrize("max_len", [1, 100000])
+@pytest.mark.parametrize("H,kv,new,hd", SHAPES)
+def test_attn_a_query_that_is_no_number(dev, H, kv, new, hd, max_len):
+    """NaN, infinities and values at the end of bf16 in one query head's row: the other rows and heads keep their bits."""
+    from grove_amd import ops
+    lens = [300, 80, 40]
+    c, q, cu, kv_len, ref = check_attn(dev, lens, [new] * 3, H, kv, hd, 16, seed=hd + H + 9, max_len=max_len)
+    keep = torch.ones(3 * new, H, dtype=torch.bool)
+    keep[new, H - 1] = False
+    for bad in (math.nan, math.inf, -math.inf, 3e38):
+        x = q.clone()
+        x[new, H - 1, 5] = bad
+        r = ops.kv4_attn(x.to(dev), c.cache, c.table, kv_len, cu, new, hd ** -0.5, max_len=max_len)
+        assert torch.equal(r.view(3 * new, H, hd)[keep], ref.view(3 * new, H, hd)[keep]), bad
+        if bad != 3e38:
+            assert r.view(3 * new, H, hd)[new, H - 1].isnan().all(), bad
